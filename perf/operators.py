@@ -89,8 +89,9 @@ def draw(rng):
         if not odd:
             hidden = hidden // 8 * 8
         ffn, kv = int(hidden * rng.uniform(2.0, 3.5)), max(1, hidden // rng.choice([1, 2, 4, 8]))
-        layers = _spread(rng, 1, max(1, min(60, int(6e8 / (hidden * (2 * hidden + 2 * kv + 3 * ffn))))))
-        return _clip(None, hidden, layers, ffn, rng.choice([0, _spread(rng, 100, max(101, min(92544, int(1e8 / hidden))))]), kv, grads=rng.choice(["bf16", "fp32", "mixed"]),
+        layers = _spread(rng, 1, max(1, min(60, int(4.5e8 / (hidden * (2 * hidden + 2 * kv + 3 * ffn))))))
+        vocab = rng.choice([0, _spread(rng, 100, max(101, min(92544, int(7e7 / hidden))))])
+        return _clip(None, hidden, layers, ffn, vocab, kv, grads=rng.choice(["bf16", "fp32", "mixed"]),
                      out=rng.choice(["bf16", "fp32"]), form=rng.choice(["clip", "clip", "norm"]), odd=odd, max_norm=rng.choice([0.5, 1.0, 1e6]))
     vocab = rng.choice([32000, 92544, 103168, _spread(rng, 500, 131072), _spread(rng, 500, 131072)])
     dtype = rng.choice(["bf16", "bf16", "fp32"])
@@ -100,8 +101,8 @@ def draw(rng):
     if op == "preference":
         seqs = max(2, seqs // 2 * 2)
         average = rng.random() < 0.4
-        extra = _pref(kind=rng.choice(["sigmoid", "sigmoid", "hinge", "ipo"]), average=average, reference=not average or rng.random() < 0.5, beta=rng.choice([0.05, 0.1, 0.5, 2.0]),
-                      train=rng.random() < 0.75, empty=rng.random() < 0.2)
+        extra = _pref(kind=rng.choice(["sigmoid", "sigmoid", "hinge", "ipo"]), average=average, reference=not average or rng.random() < 0.5,
+                      beta=rng.choice([0.05, 0.1, 0.5, 2.0]), train=rng.random() < 0.75, empty=rng.random() < 0.2)
         if extra["kind"] == "sigmoid":
             extra["smoothing"] = rng.choice([0.0, 0.1])
         if extra["kind"] != "ipo":
