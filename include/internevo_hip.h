@@ -486,6 +486,68 @@ int ie_tune_gemm_queue_memset(int on);
  * sums against the unsplit product.  The workspace is used in stream order by every such product: one stream at a time. */
 int ie_gemm_set_wgrad_ksplit_workspace(void* ws, int64_t bytes);
 
+/* ------------------------------------------------------------------------------------------------
+ * Losses of preference and policy training over the same logits the cross-entropy reads (the reference trains on the cross-entropy only:
+ * internlm/model/losses/ce_loss.py:26-58; these stand beside it and have no counterpart there).
+ *   z = logits[t] * inv_temperature;  lse[t] = log sum_j exp z_j;  logp[t] = z[labels[t]] - lse[t]
+ * logits [rows, vocab] bf16 or fp32, row stride ld, any element address; labels int64 [rows].  A row whose label is ignore_index or lies outside [0, vocab) is
+ * masked: its logits are not read, its logp, lse and coef are 0, its gradient row is zeros.  Every [rows] output is written for all rows.
+ * ld >= vocab, rows < 2^31, vocab <= 2^30.  No workgroup waits for another and no sum uses atomics: results repeat bit for bit.
+ *
+ * ie_logprob_fwd: logp, lse (fp32 [rows]).
+ * ie_logprob_bwd: dlogits[t, j] = g_t ([j == labels[t]] - exp(z_j - lse[t])), g_t = coef[t] * dloss_mul * inv_temperature * (dloss ? *dloss : 1);
+ *   coef fp32 [rows] = d loss / d logp, dloss a DEVICE scalar (the loss scale) or NULL.  dlogits has the logits' type and a row stride of its own; it is the
+ *   logits themselves (same address, same stride) or does not overlap them.  A row with g_t = 0 is written as zeros without a look at its logits.
+ *
+ * ie_preference_loss_fwd: cu_seqlens int32 [2 pairs + 1] packs chosen answer 2p and rejected answer 2p + 1; offsets are clamped to [0, rows], rows outside every
+ *   sequence are in no sum.  l_s = sum (average: mean; 0 for an answer without a token) of logp over the rows of sequence s that have a label,
+ *   h_p = (l_2p - ref_2p) - (l_2p+1 - ref_2p+1) (ref_logps fp32 [2 pairs], NULL = 0), z = beta h - margin;
+ *     IE_PREF_SIGMOID  -(1 - s) log sigmoid(z) - s log sigmoid(-z)   (s = label_smoothing in [0, 0.5])
+ *     IE_PREF_HINGE    max(0, 1 - z)
+ *     IE_PREF_IPO      (h - 1 / (2 beta))^2                          (no margin)
+ *   loss[0] = mean over the pairs; rewards [2 pairs] = beta (l - ref); seq_logps [2 pairs] = l; coef [rows] = d loss / d logp for ie_logprob_bwd.
+ *   Sums and losses are formed in 64 bits.  workspace: ie_preference_loss_workspace(pairs) bytes, 8-byte aligned, for this call only.
+ *
+ * ie_policy_loss: r = exp(logp - old_logps), loss term -min(r A, clamp(r, 1 - clip_low, 1 + clip_high) A) + kl_coef (exp(q) - q - 1), q = ref_logps - logp
+ *   (ref_logps NULL: no KL term, kl_coef must be 0); old_logps, advantages, ref_logps fp32 [rows], not looked at in masked rows.  Weights: cu_seqlens NULL
+ *   (seqs = 0): 1 / N over the N rows with a label; cu_seqlens int32 [seqs + 1]: 1 / (seqs n_s) for the n_s labelled rows of sequence s, 0 outside every sequence.
+ *   stats[4] = {loss, policy term, KL, share of clipped rows} under those weights (all 0 for a batch without a label); logp, lse, coef as above.
+ *   dlogits and dloss given: the gradient too, in the same pass over the logits (dlogits as in ie_logprob_bwd); both NULL: forward only, ie_logprob_bwd follows.
+ *   workspace: ie_policy_loss_workspace(rows, seqs) bytes, 4-byte aligned, for this call only.
+ * ---------------------------------------------------------------------------------------------- */
+#define IE_PREF_SIGMOID 0
+#define IE_PREF_HINGE 1
+#define IE_PREF_IPO 2
+int ie_logprob_fwd(const void* logits, int dtype, int64_t ld, const int64_t* labels, float* logp, float* lse, int64_t rows, int64_t vocab,
+                   int64_t ignore_index, float inv_temperature, void* stream);
+int ie_logprob_bwd(const void* logits, int dtype, int64_t ld, void* dlogits, int64_t ldd, const int64_t* labels, const float* lse, const float* coef,
+                   const float* dloss, float dloss_mul, int64_t rows, int64_t vocab, int64_t ignore_index, float inv_temperature, void* stream);
+int64_t ie_preference_loss_workspace(int64_t pairs);
+int ie_preference_loss_fwd(const void* logits, int dtype, int64_t ld, const int64_t* labels, const int32_t* cu_seqlens, const float* ref_logps, int kind,
+                           double beta, double label_smoothing, double margin, int average, float* loss, float* rewards, float* seq_logps, float* logp,
+                           float* lse, float* coef, void* workspace, int64_t rows, int64_t vocab, int64_t pairs, int64_t ignore_index,
+                           float inv_temperature, void* stream);
+int64_t ie_policy_loss_workspace(int64_t rows, int64_t seqs);
+int ie_policy_loss(const void* logits, int dtype, int64_t ld, void* dlogits, int64_t ldd, const int64_t* labels, const float* old_logps,
+                   const float* advantages, const float* ref_logps, const int32_t* cu_seqlens, int64_t seqs, float clip_low, float clip_high,
+                   float kl_coef, const float* dloss, float dloss_mul, float* stats, float* logp, float* lse, float* coef, void* workspace,
+                   int64_t rows, int64_t vocab, int64_t ignore_index, float inv_temperature, void* stream);
+
+/* ------------------------------------------------------------------------------------------------
+ * Norm and clipping over a LIST of n gradient tensors (compute_norm / clip over parameter lists, internlm/solver/optimizer/utils.py:191-204,330-380; ie_sumsq_*
+ * above takes one tensor a launch and squares in fp32).  ptrs, numels, dtypes are HOST arrays, read before the call returns (the launches carry them as
+ * arguments: a captured graph keeps them).  Tensors are contiguous, of any length (0 too) and any element address.
+ * ie_grad_norm: norm[0] = sqrt(sum of all squares), squares and sums in 64 bits in a fixed order (no overflow before the norm itself leaves fp32).
+ *   workspace: ie_grad_norm_workspace(n) bytes, 8-byte aligned, for this call only.
+ * ie_grad_clip: out_i = g_i * c, c = min(1, max_norm / (norm[0] + 1e-6)), with norm as ie_grad_norm left it on the device (torch.nn.utils.clip_grad_norm_'s rule:
+ *   an infinite norm gives c = 0, a NaN one c = NaN).  outs NULL: in place (nothing is moved when c = 1; tensors must not overlap); else outs[i] of out_dtypes[i],
+ *   apart from every other tensor of the call or the same one as ptrs[i].
+ * ---------------------------------------------------------------------------------------------- */
+int64_t ie_grad_norm_workspace(int64_t n);
+int ie_grad_norm(const void* const* ptrs, const int64_t* numels, const int* dtypes, int64_t n, void* workspace, float* norm, void* stream);
+int ie_grad_clip(const void* const* ptrs, const int64_t* numels, const int* dtypes, void* const* outs, const int* out_dtypes, int64_t n,
+                 const float* norm, double max_norm, void* stream);
+
 /* Diagnostic: runs one v_mfma_f32_32x32x16_bf16 with A[i][k], B[k][j] taken from a[32*16], b[16*32]
  * (row-major, bf16) using the operand/accumulator lane maps the kernels assume, writes c[32*32] fp32.
  * Lets the test-suite pin the fragment layout on real hardware. */

@@ -5,6 +5,8 @@ device pointers + sizes + ``torch.cuda.current_stream().cuda_stream`` to libinte
 ``InternEvoHipError`` on a non-zero return code.  There is no CPU / eager fallback: a tensor that is not
 on a HIP device is a ``ValueError``.
 """
+import array
+import collections
 import ctypes
 import math
 
@@ -290,6 +292,235 @@ def ce_bwd(logits, labels, lse, dloss, count, dloss_mul=1.0, ignore_index=-100, 
     check(_L().ie_ce_bwd(_p(logits), _p(dlogits), _dt(logits), ld, _p(labels), _p(lse), _p(dloss), dloss_mul, _p(count), rows, V,
                          ignore_index, label_smoothing, _stream()), "ie_ce_bwd")
     return dlogits
+
+
+# ------------------------------------------------------------------------------------------ preference / policy losses
+PreferenceLoss = collections.namedtuple("PreferenceLoss", "loss rewards seq_logps logp lse coef")
+PolicyLoss = collections.namedtuple("PolicyLoss", "loss stats logp lse coef")
+_PREFERENCE_KINDS = {"sigmoid": 0, "hinge": 1, "ipo": 2}
+
+
+def _on_current_device(*tensors):
+    """The kernels run on the current device's current stream: a tensor elsewhere is refused, not fetched."""
+    dev = tensors[0].device
+    for t in tensors:
+        if t is not None and t.device != dev:
+            raise ValueError(f"tensors on {dev} and {t.device} in one call")
+    if dev.type == "cuda" and dev.index != torch.cuda.current_device():
+        raise ValueError(f"tensors on {dev}, current device cuda:{torch.cuda.current_device()}: switch with torch.cuda.device")
+
+
+def _logit_rows(logits, name="logits"):
+    """(rows, vocab, row stride) of a 2-D tensor with unit column stride."""
+    if logits.dim() != 2 or (logits.stride(1) != 1 and logits.shape[1] > 1):
+        raise ValueError(f"{name}: expected a 2-D tensor with unit column stride")
+    rows, vocab = logits.shape
+    if vocab == 0:
+        raise ValueError(f"{name}: no columns")
+    return rows, vocab, logits.stride(0) if rows > 1 else max(vocab, logits.stride(0))
+
+
+def _row_vector(t, rows, dtype, name):
+    if t.shape != (rows,) or t.dtype != dtype or not t.is_contiguous():
+        raise ValueError(f"{name}: expected a contiguous {dtype} tensor of shape ({rows},), got {t.dtype} {tuple(t.shape)}")
+
+
+def _scalar(t, name):
+    if t.dtype != torch.float32 or t.numel() != 1:
+        raise ValueError(f"{name}: expected one fp32 value on the device")
+
+
+def _inv_temperature(temperature):
+    if not (0.0 < temperature < math.inf):
+        raise ValueError(f"the temperature must be positive and finite, not {temperature}")
+    return 1.0 / temperature
+
+
+def _dlogits_for(logits, dlogits, rows, vocab):
+    if dlogits is None:
+        dlogits = logits
+    if dlogits.shape != logits.shape or dlogits.dtype != logits.dtype:
+        raise ValueError("dlogits: shape and type must be the logits'")
+    return dlogits, _logit_rows(dlogits, "dlogits")[2]
+
+
+def token_logprobs(logits, labels, ignore_index=-100, temperature=1.0):
+    """logits [rows, V] (bf16|fp32, row stride arbitrary), labels int64 [rows] -> (logp, lse) fp32 [rows]: the log-probability of every row's label under
+    softmax(logits / temperature) and the row's log-sum-exp.  Rows whose label is ignore_index or no column are masked: both values are 0."""
+    rows, V, ld = _logit_rows(logits)
+    _row_vector(labels, rows, torch.int64, "labels")
+    inv = _inv_temperature(temperature)
+    dt = _dt(logits)
+    _on_current_device(logits, labels)
+    logp = torch.empty(rows, dtype=torch.float32, device=logits.device)
+    lse = torch.empty(rows, dtype=torch.float32, device=logits.device)
+    check(_L().ie_logprob_fwd(_p(logits), dt, ld, _p(labels), _p(logp), _p(lse), rows, V, ignore_index, inv, _stream()), "ie_logprob_fwd")
+    return logp, lse
+
+
+def token_logprobs_bwd(logits, labels, lse, dlogp, dloss=None, dloss_mul=1.0, ignore_index=-100, temperature=1.0, dlogits=None):
+    """Gradient in the logits (in place over them when dlogits is None) of a loss with d loss / d logp = dlogp fp32 [rows]; lse as token_logprobs gave it for
+    the same logits, labels and temperature.  dloss (optional, a device scalar: the loss scale) and dloss_mul are factors.  Masked rows are written as zeros."""
+    rows, V, ld = _logit_rows(logits)
+    _row_vector(labels, rows, torch.int64, "labels")
+    _row_vector(lse, rows, torch.float32, "lse")
+    _row_vector(dlogp, rows, torch.float32, "dlogp")
+    if dloss is not None:
+        _scalar(dloss, "dloss")
+    inv = _inv_temperature(temperature)
+    dlogits, ldd = _dlogits_for(logits, dlogits, rows, V)
+    dt = _dt(logits)
+    _on_current_device(logits, labels, lse, dlogp, dloss, dlogits)
+    check(_L().ie_logprob_bwd(_p(logits), dt, ld, _p(dlogits), ldd, _p(labels), _p(lse), _p(dlogp), _p(dloss), dloss_mul, rows, V, ignore_index, inv, _stream()),
+          "ie_logprob_bwd")
+    return dlogits
+
+
+def preference_loss_fwd(logits, labels, cu_seqlens, ref_logps=None, beta=0.1, kind="sigmoid", label_smoothing=0.0, margin=0.0, average=False, ignore_index=-100,
+                        temperature=1.0):
+    """Paired log-ratio loss over packed answers: cu_seqlens int32 [2 P + 1] on the device, answer 2p chosen over answer 2p + 1.  ref_logps fp32 [2 P]: the
+    reference model's summed (average: mean) log-probabilities, None = no reference.  kind "sigmoid" (label_smoothing: probability that a pair is the wrong
+    way round), "hinge" or "ipo" (formulas: include/internevo_hip.h).
+    Returns PreferenceLoss(loss [1], rewards [P, 2], seq_logps [2 P], logp, lse, coef [rows]), all fp32; hand it to preference_loss_bwd."""
+    rows, V, ld = _logit_rows(logits)
+    _row_vector(labels, rows, torch.int64, "labels")
+    seqs = cu_seqlens.numel() - 1
+    if seqs < 2 or seqs % 2:
+        raise ValueError(f"cu_seqlens: 2 P + 1 offsets of P pairs expected, got {seqs + 1}")
+    _row_vector(cu_seqlens, seqs + 1, torch.int32, "cu_seqlens")
+    if ref_logps is not None:
+        _row_vector(ref_logps, seqs, torch.float32, "ref_logps")
+    if kind not in _PREFERENCE_KINDS:
+        raise ValueError(f"kind: one of {sorted(_PREFERENCE_KINDS)}, not {kind!r}")
+    inv = _inv_temperature(temperature)
+    dt = _dt(logits)
+    _on_current_device(logits, labels, cu_seqlens, ref_logps)
+    L, dev = _L(), logits.device
+    per_row = torch.empty((3, rows), dtype=torch.float32, device=dev)
+    per_seq = torch.empty((2, seqs), dtype=torch.float32, device=dev)
+    loss = torch.empty(1, dtype=torch.float32, device=dev)
+    ws = torch.empty(L.ie_preference_loss_workspace(seqs // 2), dtype=torch.uint8, device=dev)
+    logp, lse, coef = per_row.unbind(0)
+    rewards, seq_logps = per_seq.unbind(0)
+    check(L.ie_preference_loss_fwd(_p(logits), dt, ld, _p(labels), _p(cu_seqlens), _p(ref_logps), _PREFERENCE_KINDS[kind], beta, label_smoothing, margin,
+                                   int(bool(average)), _p(loss), _p(rewards), _p(seq_logps), _p(logp), _p(lse), _p(coef), _p(ws), rows, V, seqs // 2, ignore_index,
+                                   inv, _stream()), "ie_preference_loss_fwd")
+    return PreferenceLoss(loss, rewards.view(-1, 2), seq_logps, logp, lse, coef)
+
+
+def preference_loss_bwd(logits, labels, fwd, dloss=None, dloss_mul=1.0, ignore_index=-100, temperature=1.0, dlogits=None):
+    """Gradient of preference_loss_fwd's loss in the logits (in place over them when dlogits is None); fwd: what the forward call returned."""
+    return token_logprobs_bwd(logits, labels, fwd.lse, fwd.coef, dloss, dloss_mul, ignore_index, temperature, dlogits)
+
+
+def _policy_loss(logits, labels, old_logps, advantages, dloss, dloss_mul, dlogits, ref_logps, clip_low, clip_high, kl_coef, cu_seqlens, ignore_index, temperature):
+    rows, V, ld = _logit_rows(logits)
+    _row_vector(labels, rows, torch.int64, "labels")
+    _row_vector(old_logps, rows, torch.float32, "old_logps")
+    _row_vector(advantages, rows, torch.float32, "advantages")
+    if ref_logps is not None:
+        _row_vector(ref_logps, rows, torch.float32, "ref_logps")
+    elif kl_coef != 0.0:
+        raise ValueError("a KL term needs ref_logps")
+    seqs = 0
+    if cu_seqlens is not None:
+        seqs = cu_seqlens.numel() - 1
+        if seqs < 1:
+            raise ValueError("cu_seqlens: S + 1 offsets of S sequences expected")
+        _row_vector(cu_seqlens, seqs + 1, torch.int32, "cu_seqlens")
+    inv = _inv_temperature(temperature)
+    ldd = 0
+    if dloss is not None:
+        _scalar(dloss, "dloss")
+        dlogits, ldd = _dlogits_for(logits, dlogits, rows, V)
+    dt = _dt(logits)
+    _on_current_device(logits, labels, old_logps, advantages, ref_logps, cu_seqlens, dloss, dlogits)
+    L, dev = _L(), logits.device
+    per_row = torch.empty((3, rows), dtype=torch.float32, device=dev)
+    stats = torch.empty(4, dtype=torch.float32, device=dev)
+    ws = torch.empty(L.ie_policy_loss_workspace(rows, seqs), dtype=torch.uint8, device=dev)
+    logp, lse, coef = per_row.unbind(0)
+    check(L.ie_policy_loss(_p(logits), dt, ld, _p(dlogits), ldd, _p(labels), _p(old_logps), _p(advantages), _p(ref_logps), _p(cu_seqlens), seqs, clip_low, clip_high,
+                           kl_coef, _p(dloss), dloss_mul, _p(stats), _p(logp), _p(lse), _p(coef), _p(ws), rows, V, ignore_index, inv, _stream()), "ie_policy_loss")
+    return PolicyLoss(stats[:1], stats, logp, lse, coef), dlogits
+
+
+def policy_loss_fwd(logits, labels, old_logps, advantages, ref_logps=None, clip_low=0.2, clip_high=0.2, kl_coef=0.0, cu_seqlens=None, ignore_index=-100, temperature=1.0):
+    """Clipped policy loss with a KL term: -min(r A, clamp(r, 1 - clip_low, 1 + clip_high) A) + kl_coef (e^q - q - 1), r = exp(logp - old_logps), q = ref_logps - logp;
+    old_logps, advantages, ref_logps fp32 [rows].  Mean over the rows with a label, or -- cu_seqlens int32 [S + 1] on the device -- the mean over the sequences of
+    each one's mean.  Returns PolicyLoss(loss [1], stats [4] = loss, policy term, KL, clipped share, logp, lse, coef [rows]), all fp32."""
+    return _policy_loss(logits, labels, old_logps, advantages, None, 1.0, None, ref_logps, clip_low, clip_high, kl_coef, cu_seqlens, ignore_index, temperature)[0]
+
+
+def policy_loss_bwd(logits, labels, fwd, dloss=None, dloss_mul=1.0, ignore_index=-100, temperature=1.0, dlogits=None):
+    """Gradient of policy_loss_fwd's loss in the logits (in place over them when dlogits is None); fwd: what the forward call returned."""
+    return token_logprobs_bwd(logits, labels, fwd.lse, fwd.coef, dloss, dloss_mul, ignore_index, temperature, dlogits)
+
+
+def policy_loss_fwd_bwd(logits, labels, old_logps, advantages, dloss, dloss_mul=1.0, dlogits=None, ref_logps=None, clip_low=0.2, clip_high=0.2, kl_coef=0.0,
+                        cu_seqlens=None, ignore_index=-100, temperature=1.0):
+    """policy_loss_fwd and its gradient times dloss (a device scalar: the loss scale) * dloss_mul in one pass over the logits -> (PolicyLoss, dlogits), dlogits
+    in place over the logits when None is given.  coef is d loss / d logp without the factors."""
+    if dloss is None:
+        raise ValueError("policy_loss_fwd_bwd: dloss (one fp32 value on the device) is needed")
+    return _policy_loss(logits, labels, old_logps, advantages, dloss, dloss_mul, dlogits, ref_logps, clip_low, clip_high, kl_coef, cu_seqlens, ignore_index, temperature)
+
+
+# ------------------------------------------------------------------------------------------ norm and clipping of a list of gradients
+def _tensor_list(tensors, what):
+    """Host arrays (addresses, lengths, types) of a list of contiguous bf16 / fp32 tensors."""
+    for t in tensors:
+        if not t.is_contiguous():
+            raise ValueError(f"{what}: every tensor must be contiguous")
+    return (array.array("q", [t.data_ptr() for t in tensors]), array.array("q", [t.numel() for t in tensors]), array.array("i", [_dt(t) for t in tensors]))
+
+
+def _addr(a):
+    return ctypes.c_void_p(a.buffer_info()[0])
+
+
+def grad_norm(tensors):
+    """L2 norm over a list of bf16 / fp32 tensors of any lengths -> fp32[1] on the device; squares and sums in 64 bits, fixed order."""
+    tensors = list(tensors)
+    if not tensors:
+        raise ValueError("grad_norm: an empty list")
+    return _grad_norm(tensors, _tensor_list(tensors, "grad_norm"))
+
+
+def _grad_norm(tensors, lists):
+    _on_current_device(*tensors)
+    _p(tensors[0])   # (refuses host tensors)
+    L, dev, n = _L(), tensors[0].device, len(tensors)
+    ws = torch.empty(L.ie_grad_norm_workspace(n), dtype=torch.uint8, device=dev)
+    norm = torch.empty(1, dtype=torch.float32, device=dev)
+    ptrs, numels, dtypes = lists
+    check(L.ie_grad_norm(_addr(ptrs), _addr(numels), _addr(dtypes), n, _p(ws), _p(norm), _stream()), "ie_grad_norm")
+    return norm
+
+
+def clip_grad_norm_(tensors, max_norm, out=None):
+    """Scales the gradients by min(1, max_norm / (norm + 1e-6)) (torch.nn.utils.clip_grad_norm_'s rule, its non-finite norms too) and returns their norm before that,
+    fp32[1] on the device; no host synchronisation.  In place, or into `out`: a list of contiguous tensors of the same lengths, bf16 or fp32 (the optimizer's fp32
+    gradients), apart from the inputs.  A tensor named twice, or overlapping another one that is written, is refused."""
+    tensors = list(tensors)
+    if not tensors:
+        raise ValueError("clip_grad_norm_: an empty list")
+    if not max_norm >= 0:
+        raise ValueError(f"clip_grad_norm_: max_norm must not be negative ({max_norm})")
+    lists = _tensor_list(tensors, "clip_grad_norm_")
+    optrs = odtypes = None
+    if out is not None:
+        out = list(out)
+        optrs, onumels, odtypes = _tensor_list(out, "clip_grad_norm_: out")
+        if onumels != lists[1]:
+            raise ValueError("clip_grad_norm_: out must hold one tensor of the same length for every input")
+        _on_current_device(tensors[0], *out)
+    norm = _grad_norm(tensors, lists)
+    ptrs, numels, dtypes = lists
+    none = ctypes.c_void_p(0)
+    check(_L().ie_grad_clip(_addr(ptrs), _addr(numels), _addr(dtypes), _addr(optrs) if out is not None else none, _addr(odtypes) if out is not None else none,
+                            len(tensors), _p(norm), float(max_norm), _stream()), "ie_grad_clip")
+    return norm
 
 
 # ------------------------------------------------------------------------------------------ L2 norm
