@@ -513,40 +513,40 @@ int ie_gemm_set_wgrad_ksplit_workspace(void* ws, int64_t bytes);
  *   (seqs = 0): 1 / N over the N rows with a label; cu_seqlens int32 [seqs + 1]: 1 / (seqs n_s) for the n_s labelled rows of sequence s, 0 outside every sequence.
  *   stats[4] = {loss, policy term, KL, share of clipped rows} under those weights (all 0 for a batch without a label); logp, lse, coef as above.
  *   dlogits and dloss given: the gradient too, in the same pass over the logits (dlogits as in ie_logprob_bwd); both NULL: forward only, ie_logprob_bwd follows.
- *   workspace: ie_policy_loss_workspace(rows, seqs) bytes, 4-byte aligned, for this call only.
+ *   workspace: ie_policy_loss_workspace(rows, seqs) bytes, 16-byte aligned, for this call only.
  * ---------------------------------------------------------------------------------------------- */
 #define IE_PREF_SIGMOID 0
 #define IE_PREF_HINGE 1
 #define IE_PREF_IPO 2
 int ie_logprob_fwd(const void* logits, int dtype, int64_t ld, const int64_t* labels, float* logp, float* lse, int64_t rows, int64_t vocab,
-                   int64_t ignore_index, float inv_temperature, void* stream);
+                   int64_t ignore_index, double inv_temperature, void* stream);
 int ie_logprob_bwd(const void* logits, int dtype, int64_t ld, void* dlogits, int64_t ldd, const int64_t* labels, const float* lse, const float* coef,
-                   const float* dloss, float dloss_mul, int64_t rows, int64_t vocab, int64_t ignore_index, float inv_temperature, void* stream);
+                   const float* dloss, float dloss_mul, int64_t rows, int64_t vocab, int64_t ignore_index, double inv_temperature, void* stream);
 int64_t ie_preference_loss_workspace(int64_t pairs);
 int ie_preference_loss_fwd(const void* logits, int dtype, int64_t ld, const int64_t* labels, const int32_t* cu_seqlens, const float* ref_logps, int kind,
                            double beta, double label_smoothing, double margin, int average, float* loss, float* rewards, float* seq_logps, float* logp,
                            float* lse, float* coef, void* workspace, int64_t rows, int64_t vocab, int64_t pairs, int64_t ignore_index,
-                           float inv_temperature, void* stream);
+                           double inv_temperature, void* stream);
 int64_t ie_policy_loss_workspace(int64_t rows, int64_t seqs);
 int ie_policy_loss(const void* logits, int dtype, int64_t ld, void* dlogits, int64_t ldd, const int64_t* labels, const float* old_logps,
                    const float* advantages, const float* ref_logps, const int32_t* cu_seqlens, int64_t seqs, float clip_low, float clip_high,
                    float kl_coef, const float* dloss, float dloss_mul, float* stats, float* logp, float* lse, float* coef, void* workspace,
-                   int64_t rows, int64_t vocab, int64_t ignore_index, float inv_temperature, void* stream);
+                   int64_t rows, int64_t vocab, int64_t ignore_index, double inv_temperature, void* stream);
 
 /* ------------------------------------------------------------------------------------------------
  * Norm and clipping over a LIST of n gradient tensors (compute_norm / clip over parameter lists, internlm/solver/optimizer/utils.py:191-204,330-380; ie_sumsq_*
  * above takes one tensor a launch and squares in fp32).  ptrs, numels, dtypes are HOST arrays, read before the call returns (the launches carry them as
  * arguments: a captured graph keeps them).  Tensors are contiguous, of any length (0 too) and any element address.
  * ie_grad_norm: norm[0] = sqrt(sum of all squares), squares and sums in 64 bits in a fixed order (no overflow before the norm itself leaves fp32).
- *   workspace: ie_grad_norm_workspace(n) bytes, 8-byte aligned, for this call only.
- * ie_grad_clip: out_i = g_i * c, c = min(1, max_norm / (norm[0] + 1e-6)), with norm as ie_grad_norm left it on the device (torch.nn.utils.clip_grad_norm_'s rule:
- *   an infinite norm gives c = 0, a NaN one c = NaN).  outs NULL: in place (nothing is moved when c = 1; tensors must not overlap); else outs[i] of out_dtypes[i],
- *   apart from every other tensor of the call or the same one as ptrs[i].
+ *   workspace: ie_grad_norm_workspace(n) bytes, 8-byte aligned, for this call only (both entries).
+ * ie_grad_clip: norm[0] the same, then out_i = g_i * c, c = min(1, max_norm / (norm[0] + 1e-6)) (torch.nn.utils.clip_grad_norm_'s rule: an infinite norm gives
+ *   c = 0, a NaN one c = NaN).  outs NULL: in place (nothing is moved when c = 1; tensors must not overlap); else outs[i] of out_dtypes[i] and numels[i] elements,
+ *   apart from every other tensor of the call, or the same one as ptrs[i].
  * ---------------------------------------------------------------------------------------------- */
 int64_t ie_grad_norm_workspace(int64_t n);
 int ie_grad_norm(const void* const* ptrs, const int64_t* numels, const int* dtypes, int64_t n, void* workspace, float* norm, void* stream);
-int ie_grad_clip(const void* const* ptrs, const int64_t* numels, const int* dtypes, void* const* outs, const int* out_dtypes, int64_t n,
-                 const float* norm, double max_norm, void* stream);
+int ie_grad_clip(const void* const* ptrs, const int64_t* numels, const int* dtypes, void* const* outs, const int* out_dtypes, int64_t n, double max_norm,
+                 void* workspace, float* norm, void* stream);
 
 /* Diagnostic: runs one v_mfma_f32_32x32x16_bf16 with A[i][k], B[k][j] taken from a[32*16], b[16*32]
  * (row-major, bf16) using the operand/accumulator lane maps the kernels assume, writes c[32*32] fp32.

@@ -149,15 +149,15 @@ SIGNATURES = {
     "ie_flash_attn_bwd_spill_bytes": (I64, [I, I, I, I]),
     "ie_flash_attn_bwd_set_spill": (I, [P, I64]),
     "ie_flash_attn_bwd_workspace": (I64, [I64, I, I, I]),
-    "ie_logprob_fwd": (I, [P, I, I64, P, P, P, I64, I64, I64, F, P]),
-    "ie_logprob_bwd": (I, [P, I, I64, P, I64, P, P, P, P, F, I64, I64, I64, F, P]),
+    "ie_logprob_fwd": (I, [P, I, I64, P, P, P, I64, I64, I64, Dbl, P]),
+    "ie_logprob_bwd": (I, [P, I, I64, P, I64, P, P, P, P, F, I64, I64, I64, Dbl, P]),
     "ie_preference_loss_workspace": (I64, [I64]),
-    "ie_preference_loss_fwd": (I, [P, I, I64, P, P, P, I, Dbl, Dbl, Dbl, I, P, P, P, P, P, P, P, I64, I64, I64, I64, F, P]),
+    "ie_preference_loss_fwd": (I, [P, I, I64, P, P, P, I, Dbl, Dbl, Dbl, I, P, P, P, P, P, P, P, I64, I64, I64, I64, Dbl, P]),
     "ie_policy_loss_workspace": (I64, [I64, I64]),
-    "ie_policy_loss": (I, [P, I, I64, P, I64, P, P, P, P, P, I64, F, F, F, P, F, P, P, P, P, P, I64, I64, I64, F, P]),
+    "ie_policy_loss": (I, [P, I, I64, P, I64, P, P, P, P, P, I64, F, F, F, P, F, P, P, P, P, P, I64, I64, I64, Dbl, P]),
     "ie_grad_norm_workspace": (I64, [I64]),
     "ie_grad_norm": (I, [P, P, P, I64, P, P, P]),
-    "ie_grad_clip": (I, [P, P, P, P, P, I64, P, Dbl, P]),
+    "ie_grad_clip": (I, [P, P, P, P, P, I64, Dbl, P, P, P]),
     "ie_mfma_probe": (I, [P, P, P, P]),
 }
 

@@ -21,6 +21,7 @@ template <bool BF> struct Elem;
 template <> struct Elem<true> {
     typedef bf16_t T;
     static constexpr int N = 8;
+    static __device__ __forceinline__ u32x4 ninf() { return u32x4{0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u}; }
     static __device__ __forceinline__ float get(const T* p) { return bf2f(*p); }
     static __device__ __forceinline__ void put(T* p, float f) { *p = f2bf(f); }
     static __device__ __forceinline__ void unpack(const u32x4& v, float* f) {
@@ -37,6 +38,7 @@ template <> struct Elem<true> {
 template <> struct Elem<false> {
     typedef float T;
     static constexpr int N = 4;
+    static __device__ __forceinline__ u32x4 ninf() { return u32x4{0xff800000u, 0xff800000u, 0xff800000u, 0xff800000u}; }
     static __device__ __forceinline__ float get(const T* p) { return *p; }
     static __device__ __forceinline__ void put(T* p, float f) { *p = f; }
     static __device__ __forceinline__ void unpack(const u32x4& v, float* f) {
@@ -53,7 +55,15 @@ template <> struct Elem<false> {
 
 __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
 
-constexpr float kLog2e = 1.44269504088896341f;
+constexpr double kLog2e = 1.44269504088896340736;
+constexpr double kLn2 = 0.693147180559945309417;
+
+// S: past the caches (non-temporal), for logits or gradients larger than the last-level cache
+template <bool S> __device__ __forceinline__ u32x4 ldv(const void* p) { return S ? __builtin_nontemporal_load((const u32x4_any*)p) : *(const u32x4_any*)p; }
+template <bool S> __device__ __forceinline__ void stv(void* p, const u32x4& v) {
+    if (S) __builtin_nontemporal_store(v, (u32x4_any*)p);
+    else *(u32x4_any*)p = v;
+}
 
 // Maximum m of a row and s = sum 2^((x - m) k), k = log2(e) / tau, in one pass: 2^((m_old - m_new) k) rescales what was summed before a new maximum.  The difference
 // is taken before the product: it is exact next to the maximum, and logits masked by the type's lowest value cannot overflow into inf - inf.  While nothing but
@@ -63,36 +73,83 @@ __device__ __forceinline__ float rescale(float m_old, float m_new, float k) { re
 
 struct RowStat {
     float m, s;
-    float log_sum;     // log sum exp((x - m) / tau)
-    __device__ __forceinline__ float lse(float inv_tau) const { return fmaf(m, inv_tau, log_sum); }
+    // log sum exp((x - m) / tau): the exponent of s apart, so that only the logarithm of a number next to 1 is rounded to 32 bits
+    __device__ __forceinline__ double log_sum() const {
+        int e;
+        float f = frexpf(s, &e);
+        if (!(f > 0.f) || f == INFINITY) return (double)logf(s);
+        if (f < 0.70710678f) { f *= 2.f; --e; }
+        return (double)e * kLn2 + (double)logf(f);
+    }
+    __device__ __forceinline__ double lse(double inv_tau) const { return (double)m * inv_tau + log_sum(); }
+    __device__ __forceinline__ double logp(float x, double inv_tau) const { return ((double)x - (double)m) * inv_tau - log_sum(); }
 };
 
-template <bool BF, int NT>
-__device__ RowStat row_stat(const typename Elem<BF>::T* __restrict__ x, int vocab, float k, float* scratch) {
+// (m, s) of every thread -> of the workgroup; every thread returns the same.  sh: 2 NT / 64 floats.
+template <int NT>
+__device__ __forceinline__ RowStat join_stats(float m, float s, float k, float* sh) {
+    constexpr int NW = NT / 64;
+    const float wm = wave_max(m);
+    s = wave_sum(s * rescale(m, wm, k));
+    if (NW == 1) return {wm, s};
+    if ((threadIdx.x & 63) == 0) { sh[threadIdx.x >> 6] = wm; sh[NW + (threadIdx.x >> 6)] = s; }
+    __syncthreads();
+    m = sh[threadIdx.x & (NW - 1)];
+    float b = m;
+#pragma unroll
+    for (int o = NW / 2; o > 0; o >>= 1) b = fmaxf(b, __shfl_xor(b, o, 64));
+    s = sh[NW + (threadIdx.x & (NW - 1))] * rescale(m, b, k);
+#pragma unroll
+    for (int o = NW / 2; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
+    return {b, s};
+}
+
+template <bool BF>
+__device__ __forceinline__ void add_values(const float* v, int n, float k, float& m, float& s) {
+    float c = v[0];
+#pragma unroll
+    for (int e = 1; e < n; ++e) c = fmaxf(c, v[e]);
+    if (c > m) { s *= rescale(m, c, k); m = c; }
+    const float r = max_ref(m);
+#pragma unroll
+    for (int e = 0; e < n; ++e) s += exp2_((v[e] - r) * k);
+}
+
+// One pass over the row, U 16-byte loads a thread in flight.
+template <bool BF, int NT, int U, bool S>
+__device__ __forceinline__ RowStat row_stat(const typename Elem<BF>::T* __restrict__ x, int vocab, float k, float* sh) {
     constexpr int N = Elem<BF>::N;
     float m = -INFINITY, s = 0.f;
     const int nv = vocab / N;
-    for (int i = threadIdx.x; i < nv; i += NT) {
-        float v[N];
-        Elem<BF>::unpack(*(const u32x4_any*)(x + (int64_t)i * N), v);
-        float cm = v[0];
+    int i = threadIdx.x;
+    for (; i + (U - 1) * NT < nv; i += U * NT) {
+        u32x4 w[U];
 #pragma unroll
-        for (int e = 1; e < N; ++e) cm = fmaxf(cm, v[e]);
-        if (cm > m) { s *= rescale(m, cm, k); m = cm; }
-        const float r = max_ref(m);
+        for (int u = 0; u < U; ++u) w[u] = ldv<S>(x + (int64_t)(i + u * NT) * N);
+        float v[U * N];
 #pragma unroll
-        for (int e = 0; e < N; ++e) s += exp2_((v[e] - r) * k);
+        for (int u = 0; u < U; ++u) Elem<BF>::unpack(w[u], v + u * N);
+        add_values<BF>(v, U * N, k, m, s);
     }
-    for (int i = nv * N + threadIdx.x; i < vocab; i += NT) {
-        const float v = Elem<BF>::get(x + i);
-        if (v > m) { s *= rescale(m, v, k); m = v; }
-        s += exp2_((v - max_ref(m)) * k);
+    if (U > 1 && i < nv) {   // fewer than U vectors left: loaded together too, what is not there stays -inf
+        u32x4 w[U - 1];
+#pragma unroll
+        for (int u = 0; u < U - 1; ++u) {
+            w[u] = Elem<BF>::ninf();
+            if (i + u * NT < nv) w[u] = ldv<S>(x + (int64_t)(i + u * NT) * N);
+        }
+#pragma unroll
+        for (int u = 0; u < U - 1; ++u) {
+            float v[N];
+            Elem<BF>::unpack(w[u], v);
+            add_values<BF>(v, N, k, m, s);
+        }
     }
-    RowStat st;
-    st.m = block_max<NT / 64>(m, scratch);
-    st.s = block_sum<NT / 64>(s * rescale(m, st.m, k), scratch);
-    st.log_sum = logf(st.s);
-    return st;
+    if ((int)threadIdx.x < vocab - nv * N) {
+        const float v = Elem<BF>::get(x + nv * N + threadIdx.x);
+        add_values<BF>(&v, 1, k, m, s);
+    }
+    return join_stats<NT>(m, s, k, sh);
 }
 
 __device__ __forceinline__ bool row_label(const int64_t* labels, int64_t row, int64_t ignore_index, int vocab, int& lab) {
@@ -101,41 +158,64 @@ __device__ __forceinline__ bool row_label(const int64_t* labels, int64_t row, in
     return l != ignore_index && l >= 0 && l < vocab;
 }
 
-// d = g 1[j = label] - g_p 2^((x - m) k) for the whole row: with the row's maximum and sum g_p = g / s, with its log-sum-exp in m's place g_p = g.  The label's own
-// element is written last by the thread that owns it, from the logit it read before: dlogits may be the logits themselves.
+// The thread that writes element `lab` of a row in the loops below: its own later store puts the label's element right.
 template <bool BF, int NT>
-__device__ void row_grad(const typename Elem<BF>::T* x, typename Elem<BF>::T* d, int vocab, float k, float m, float g, float g_p, int lab) {
+__device__ __forceinline__ bool owns(int lab, int vocab) {
     constexpr int N = Elem<BF>::N;
     const int nv = vocab / N;
-    const int owner = lab < nv * N ? (lab / N) % NT : (lab - nv * N) % NT;
-    float xl = 0.f;
-    if ((int)threadIdx.x == owner) xl = Elem<BF>::get(x + lab);
-    for (int i = threadIdx.x; i < nv; i += NT) {
-        float v[N];
-        Elem<BF>::unpack(*(const u32x4_any*)(x + (int64_t)i * N), v);
-#pragma unroll
-        for (int e = 0; e < N; ++e) v[e] = -g_p * exp2_((v[e] - m) * k);
-        *(u32x4_any*)(d + (int64_t)i * N) = Elem<BF>::pack(v);
-    }
-    for (int i = nv * N + threadIdx.x; i < vocab; i += NT) Elem<BF>::put(d + i, -g_p * exp2_((Elem<BF>::get(x + i) - m) * k));
-    if ((int)threadIdx.x == owner) Elem<BF>::put(d + lab, g - g_p * exp2_((xl - m) * k));
+    return (int)threadIdx.x == (lab < nv * N ? (lab / N) % NT : lab - nv * N);
 }
 
-template <bool BF, int NT>
-__device__ void row_zero(typename Elem<BF>::T* d, int vocab) {
+template <bool BF>
+__device__ __forceinline__ u32x4 grad_vector(const u32x4& w, float k, float m, float g_p) {
+    float v[Elem<BF>::N];
+    Elem<BF>::unpack(w, v);
+#pragma unroll
+    for (int e = 0; e < Elem<BF>::N; ++e) v[e] = -g_p * exp2_((v[e] - m) * k);
+    return Elem<BF>::pack(v);
+}
+
+// d = g 1[j = label] - g_p 2^((x - m) k) for the whole row: with the row's maximum and sum g_p = g / s, with its log-sum-exp in m's place g_p = g.  xl: the label's
+// logit, read before any store (dlogits may be the logits themselves).
+template <bool BF, int NT, int U, bool S>
+__device__ __forceinline__ void row_grad(const typename Elem<BF>::T* x, typename Elem<BF>::T* d, int vocab, float k, float m, float g, float g_p, int lab, float xl) {
+    constexpr int N = Elem<BF>::N;
+    const int nv = vocab / N;
+    int i = threadIdx.x;
+    for (; i + (U - 1) * NT < nv; i += U * NT) {
+        u32x4 w[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) w[u] = ldv<S>(x + (int64_t)(i + u * NT) * N);
+#pragma unroll
+        for (int u = 0; u < U; ++u) stv<S>(d + (int64_t)(i + u * NT) * N, grad_vector<BF>(w[u], k, m, g_p));
+    }
+    u32x4 w[U - 1];
+#pragma unroll
+    for (int u = 0; u < U - 1; ++u)
+        if (i + u * NT < nv) w[u] = ldv<S>(x + (int64_t)(i + u * NT) * N);
+#pragma unroll
+    for (int u = 0; u < U - 1; ++u)
+        if (i + u * NT < nv) stv<S>(d + (int64_t)(i + u * NT) * N, grad_vector<BF>(w[u], k, m, g_p));
+    i = nv * N + threadIdx.x;
+    if (i < vocab) Elem<BF>::put(d + i, -g_p * exp2_((Elem<BF>::get(x + i) - m) * k));
+    if (owns<BF, NT>(lab, vocab)) Elem<BF>::put(d + lab, g - g_p * exp2_((xl - m) * k));
+}
+
+template <bool BF, int NT, bool S>
+__device__ __forceinline__ void row_zero(typename Elem<BF>::T* d, int vocab) {
     constexpr int N = Elem<BF>::N;
     const int nv = vocab / N;
     const u32x4 z = {0, 0, 0, 0};
-    for (int i = threadIdx.x; i < nv; i += NT) *(u32x4_any*)(d + (int64_t)i * N) = z;
-    for (int i = nv * N + threadIdx.x; i < vocab; i += NT) Elem<BF>::put(d + i, 0.f);
+    for (int i = threadIdx.x; i < nv; i += NT) stv<S>(d + (int64_t)i * N, z);
+    if (nv * N + (int)threadIdx.x < vocab) Elem<BF>::put(d + nv * N + threadIdx.x, 0.f);
 }
 
 // ------------------------------------------------------------------------------------------ log-probabilities
 // coef (may be null) is cleared: the loss kernels behind this one set it for the rows of their sequences only.
-template <bool BF, int NT>
+template <bool BF, int NT, bool S>
 __global__ __launch_bounds__(NT) void logprob_fwd_k(const void* __restrict__ logits, int64_t ld, const int64_t* __restrict__ labels, float* __restrict__ logp,
-                                                    float* __restrict__ lse, float* __restrict__ coef, int vocab, int64_t ignore_index, float inv_tau) {
-    __shared__ float scratch[NT / 64];
+                                                    float* __restrict__ lse, float* __restrict__ coef, int vocab, int64_t ignore_index, double inv_tau) {
+    __shared__ float sh[NT / 32];
     const int64_t row = blockIdx.x;
     int lab;
     if (!row_label(labels, row, ignore_index, vocab, lab)) {
@@ -143,36 +223,42 @@ __global__ __launch_bounds__(NT) void logprob_fwd_k(const void* __restrict__ log
         return;
     }
     const typename Elem<BF>::T* x = (const typename Elem<BF>::T*)logits + row * ld;
-    const RowStat st = row_stat<BF, NT>(x, vocab, inv_tau * kLog2e, scratch);
+    const float xl = Elem<BF>::get(x + lab);
+    const RowStat st = row_stat<BF, NT, 4, S>(x, vocab, (float)(inv_tau * kLog2e), sh);
     if (threadIdx.x == 0) {
-        lse[row] = st.lse(inv_tau);
-        logp[row] = (Elem<BF>::get(x + lab) - st.m) * inv_tau - st.log_sum;
+        lse[row] = (float)st.lse(inv_tau);
+        logp[row] = (float)st.logp(xl, inv_tau);
         if (coef) coef[row] = 0.f;
     }
 }
 
-template <bool BF, int NT>
+template <bool BF, int NT, int U, bool S>
 __global__ __launch_bounds__(NT) void logprob_bwd_k(const void* logits, int64_t ld, void* dlogits, int64_t ldd, const int64_t* __restrict__ labels,
                                                     const float* __restrict__ lse, const float* __restrict__ coef, const float* __restrict__ dloss, float dloss_mul,
-                                                    int vocab, int64_t ignore_index, float inv_tau) {
-    __shared__ float scratch[NT / 64];
+                                                    int vocab, int64_t ignore_index, double inv_tau) {
+    __shared__ float sh[NT / 32];
     const int64_t row = blockIdx.x;
     int lab;
     typename Elem<BF>::T* d = (typename Elem<BF>::T*)dlogits + row * ldd;
     const bool valid = row_label(labels, row, ignore_index, vocab, lab);
-    float g = valid ? coef[row] * dloss_mul * inv_tau : 0.f;
+    float g = valid ? coef[row] * dloss_mul * (float)inv_tau : 0.f;
     if (dloss) g *= dloss[0];
-    if (!valid || g == 0.f) { row_zero<BF, NT>(d, vocab); return; }
-    const float k = inv_tau * kLog2e;
+    if (!valid || g == 0.f) { row_zero<BF, NT, S>(d, vocab); return; }
+    const float k = (float)(inv_tau * kLog2e);
     const typename Elem<BF>::T* x = (const typename Elem<BF>::T*)logits + row * ld;
-    float m = lse[row] / inv_tau, g_p = g;
+    const float xl = Elem<BF>::get(x + lab);
+    // p = 2^((x - l) k), l = lse tau: what rounding l to 32 bits loses goes into the factor
+    const double l = (double)lse[row] / inv_tau;
+    float m = (float)l, g_p = g;
     if (m < -1e30f) {   // every logit at the type's lowest value or below: there the log-sum-exp cannot hold the sum beside the maximum
-        const RowStat st = row_stat<BF, NT>(x, vocab, k, scratch);
-        __syncthreads();
+        const RowStat st = row_stat<BF, NT, 4, S>(x, vocab, k, sh);
         m = st.m;
         g_p = g / st.s;
+    } else {
+        g_p *= exp2_((float)((double)m - l) * k);
     }
-    row_grad<BF, NT>(x, d, vocab, k, m, g, g_p, lab);
+    __syncthreads();   // xl is read before another wave's stores may replace it
+    row_grad<BF, NT, U, S>(x, d, vocab, k, m, g, g_p, lab, xl);
 }
 
 // ------------------------------------------------------------------------------------------ sums over a workgroup in 64 bits, fixed order
@@ -193,6 +279,8 @@ __device__ __forceinline__ void seq_range(const int32_t* cu, int64_t s, int64_t 
     begin = min(max((int64_t)cu[s], (int64_t)0), rows);
     end = min(max((int64_t)cu[s + 1], begin), rows);
 }
+
+constexpr int kSmallRows = 4096;   // rows that one workgroup finishes alone after their log-probabilities
 
 // ------------------------------------------------------------------------------------------ preference loss
 struct PrefArgs {
@@ -219,42 +307,66 @@ __device__ __forceinline__ double pair_loss(const PrefArgs& a, double h, double&
     return q * q;
 }
 
-// One workgroup per pair (sequences 2p, 2p + 1): sums of the log-probabilities in 64 bits, the pair's loss, and the coefficient of every row of the pair.
-__global__ __launch_bounds__(256) void preference_pair_k(const float* __restrict__ logp, const int64_t* __restrict__ labels, const int32_t* __restrict__ cu,
-                                                         const float* __restrict__ ref, int64_t rows, int64_t pairs, int64_t ignore_index, int vocab, PrefArgs a,
-                                                         double* __restrict__ losses, float* __restrict__ rewards, float* __restrict__ seq_logps,
-                                                         float* __restrict__ coef) {
-    __shared__ double scratch[4];
-    const int64_t p = blockIdx.x;
+struct PrefRows {
+    const float* logp;
+    const int64_t* labels;
+    const int32_t* cu;
+    const float* ref;
+    int64_t rows, pairs, ignore_index;
+    int vocab;
+    float *rewards, *seq_logps, *coef;
+};
+
+__device__ __forceinline__ bool pref_label(const PrefRows& p, int64_t t) {
+    int lab;
+    return row_label(p.labels, t, p.ignore_index, p.vocab, lab);
+}
+
+// Sequences 2i, 2i + 1 by NT threads: sums of the log-probabilities in 64 bits, the pair's loss (returned to every thread), the coefficient of every row of the pair.
+// NT = 64: the calling wave; otherwise the workgroup (scratch: NT / 64 doubles).
+template <int NT>
+__device__ __forceinline__ double preference_pair(const PrefRows& r, const PrefArgs& a, int64_t i, double* scratch) {
+    const int tid = threadIdx.x & (NT - 1);
     int64_t begin[2], end[2];
-    double l[2], n[2], gain[2];
+    double l[2], n[2];
+#pragma unroll
     for (int c = 0; c < 2; ++c) {
-        const int64_t s = 2 * p + c;
-        seq_range(cu, s, rows, begin[c], end[c]);
-        double sum = 0.0, cnt = 0.0;
-        for (int64_t t = begin[c] + threadIdx.x; t < end[c]; t += 256) {
-            int lab;
-            if (row_label(labels, t, ignore_index, vocab, lab)) { sum += (double)logp[t]; cnt += 1.0; }
-        }
-        l[c] = block_sum_d<4>(sum, scratch);
-        n[c] = block_sum_d<4>(cnt, scratch);
-        if (a.average) l[c] /= fmax(n[c], 1.0);
-        gain[c] = l[c] - (ref ? (double)ref[s] : 0.0);
-        if (threadIdx.x == 0) {
-            seq_logps[s] = (float)l[c];
-            rewards[s] = (float)(a.beta * gain[c]);
+        seq_range(r.cu, 2 * i + c, r.rows, begin[c], end[c]);
+        l[c] = 0.0;
+        int cnt = 0;
+#pragma unroll 4
+        for (int64_t t = begin[c] + tid; t < end[c]; t += NT)
+            if (pref_label(r, t)) { l[c] += (double)r.logp[t]; ++cnt; }
+        n[c] = (double)cnt;
+    }
+    double gain[2];
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+        l[c] = NT == 64 ? wave_sum_d(l[c]) : block_sum_d<NT / 64>(l[c], scratch);
+        n[c] = fmax(NT == 64 ? wave_sum_d(n[c]) : block_sum_d<NT / 64>(n[c], scratch), 1.0);
+        if (a.average) l[c] /= n[c];
+        gain[c] = l[c] - (r.ref ? (double)r.ref[2 * i + c] : 0.0);
+        if (tid == 0) {
+            r.seq_logps[2 * i + c] = (float)l[c];
+            r.rewards[2 * i + c] = (float)(a.beta * gain[c]);
         }
     }
     double slope;
     const double loss = pair_loss(a, gain[0] - gain[1], slope);
-    if (threadIdx.x == 0) losses[p] = loss;
+#pragma unroll
     for (int c = 0; c < 2; ++c) {
-        const float w = (float)((c ? -slope : slope) / (double)pairs / (a.average ? fmax(n[c], 1.0) : 1.0));
-        for (int64_t t = begin[c] + threadIdx.x; t < end[c]; t += 256) {
-            int lab;
-            if (row_label(labels, t, ignore_index, vocab, lab)) coef[t] = w;
-        }
+        const float w = (float)((c ? -slope : slope) / (double)r.pairs / (a.average ? n[c] : 1.0));
+#pragma unroll 4
+        for (int64_t t = begin[c] + tid; t < end[c]; t += NT)
+            if (pref_label(r, t)) r.coef[t] = w;
     }
+    return loss;
+}
+
+__global__ __launch_bounds__(1024) void preference_pair_k(PrefRows r, PrefArgs a, double* __restrict__ losses) {
+    __shared__ double scratch[16];
+    const double loss = preference_pair<1024>(r, a, blockIdx.x, scratch);
+    if (threadIdx.x == 0) losses[blockIdx.x] = loss;
 }
 
 __global__ __launch_bounds__(256) void preference_mean_k(const double* __restrict__ losses, int64_t pairs, float* __restrict__ loss) {
@@ -265,13 +377,33 @@ __global__ __launch_bounds__(256) void preference_mean_k(const double* __restric
     if (threadIdx.x == 0) loss[0] = (float)(v / (double)pairs);
 }
 
+constexpr int kSmallPairs = 16;   // one workgroup, a wave per pair, finishes a batch of up to this many pairs of up to kSmallRows rows in all
+
+__global__ __launch_bounds__(1024) void preference_small_k(PrefRows r, PrefArgs a, float* __restrict__ loss) {
+    __shared__ double losses[kSmallPairs];
+    const int w = threadIdx.x >> 6;
+    if (w < r.pairs) {
+        const double v = preference_pair<64>(r, a, w, nullptr);
+        if ((threadIdx.x & 63) == 0) losses[w] = v;
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        double v = 0.0;
+        for (int i = 0; i < (int)r.pairs; ++i) v += losses[i];
+        loss[0] = (float)(v / (double)r.pairs);
+    }
+}
+
 // ------------------------------------------------------------------------------------------ policy loss
+constexpr int kCountRows = 4;      // labels a thread looks at where a row's own workgroup counts
+constexpr int kSmallSeqs = 1024;   // one workgroup finishes a forward pass of up to kSmallRows rows in up to this many sequences
+
 struct PolicyArgs {
     const int64_t* labels;
     const int32_t* cu;      // null: one mean over all tokens
     const float *old_logps, *adv, *ref;   // ref null: no KL term
-    const int32_t* counts;  // tokens of every sequence, or of the whole batch
-    float* terms;           // [3][rows]: weighted surrogate, KL, clipped
+    const int32_t* counts;  // tokens of every sequence, or of the whole batch; null: the rows' own workgroups count
+    float4* terms;          // [rows]: weighted surrogate, KL, clipped
     float* coef;
     int64_t rows, seqs, ignore_index;
     int vocab;
@@ -283,41 +415,50 @@ __global__ __launch_bounds__(1024) void policy_counts_k(PolicyArgs a, int32_t* _
     __shared__ double scratch[16];
     int64_t begin = 0, end = a.rows;
     if (a.cu) seq_range(a.cu, blockIdx.x, a.rows, begin, end);
-    double n = 0.0;
+    int n = 0;
+#pragma unroll 8
     for (int64_t t = begin + threadIdx.x; t < end; t += 1024) {
         int lab;
-        n += row_label(a.labels, t, a.ignore_index, a.vocab, lab) ? 1.0 : 0.0;
+        n += row_label(a.labels, t, a.ignore_index, a.vocab, lab) ? 1 : 0;
     }
-    n = block_sum_d<16>(n, scratch);
-    if (threadIdx.x == 0) counts[blockIdx.x] = (int32_t)n;
+    const double total = block_sum_d<16>((double)n, scratch);
+    if (threadIdx.x == 0) counts[blockIdx.x] = (int32_t)total;
 }
 
-// weight of row t's term: 1 / N, or 1 / (S n_s); 0 outside every sequence.  Called by whole waves with one t.
-__device__ __forceinline__ float policy_weight(const PolicyArgs& a, int64_t t) {
-    if (!a.cu) return 1.f / (float)max(a.counts[0], 1);
-    int64_t s = 0;   // how many of cu[1..S] are <= t
-    for (int64_t i = threadIdx.x & 63; i - (int64_t)(threadIdx.x & 63) < a.seqs; i += 64) s += __popcll(__ballot(i < a.seqs && (int64_t)a.cu[i + 1] <= t));
-    if (s >= a.seqs || t < (int64_t)a.cu[0]) return 0.f;
-    return 1.f / ((float)a.seqs * (float)max(a.counts[s], 1));
+// Rows [begin, end) that row t's mean runs over, s their sequence; false outside every sequence.  Called by whole waves with one t.
+__device__ __forceinline__ bool policy_range(const PolicyArgs& a, int64_t t, int64_t& s, int64_t& begin, int64_t& end) {
+    s = 0; begin = 0; end = a.rows;
+    if (!a.cu) return true;
+    for (int64_t i = 0; i < a.seqs; i += 64) {   // how many of cu[1..S] are <= t
+        const int64_t j = i + (threadIdx.x & 63);
+        s += __popcll(__ballot(j < a.seqs && (int64_t)a.cu[min(j, a.seqs - 1) + 1] <= t));
+    }
+    if (s >= a.seqs) return false;
+    seq_range(a.cu, s, a.rows, begin, end);
+    return t >= begin && t < end;
 }
 
-// terms of one row and d loss / d logp
-__device__ __forceinline__ float policy_term(const PolicyArgs& a, int64_t t, float logp, float w) {
+// weight of a row's term: 1 / N, or 1 / (S n_s); 0 outside every sequence
+__device__ __forceinline__ float policy_weight(const PolicyArgs& a, bool inside, int n) {
+    return inside ? (float)(1.0 / ((a.cu ? (double)a.seqs : 1.0) * (double)max(n, 1))) : 0.f;
+}
+
+// terms of one row and d loss / d logp; the log-ratios are differences of 64-bit values, so that they alone are rounded
+__device__ __forceinline__ float policy_term(const PolicyArgs& a, int64_t t, double logp, float w, float4& term) {
+    term = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (w == 0.f) return 0.f;
     const float adv = a.adv[t];
-    const float ratio = expf(logp - a.old_logps[t]);
+    const float ratio = expf((float)(logp - (double)a.old_logps[t]));
     const bool clipped = (adv > 0.f && ratio > 1.f + a.high) || (adv < 0.f && ratio < 1.f - a.low);
     const float bound = adv > 0.f ? 1.f + a.high : 1.f - a.low;
     const float s = -(clipped ? bound : ratio) * adv;
     float d = clipped ? 0.f : -ratio * adv, kl = 0.f;
     if (a.ref) {
-        const float q = a.ref[t] - logp, e = expm1f(q);
+        const float q = (float)((double)a.ref[t] - logp), e = expm1f(q);
         kl = e - q;
         if (a.kl_coef > 0.f) d -= a.kl_coef * e;   // (0 * inf would turn a mere report into NaN)
     }
-    if (w == 0.f) { a.terms[t] = 0.f; a.terms[a.rows + t] = 0.f; a.terms[2 * a.rows + t] = 0.f; return 0.f; }
-    a.terms[t] = w * s;
-    a.terms[a.rows + t] = w * kl;
-    a.terms[2 * a.rows + t] = clipped ? w : 0.f;
+    term = make_float4(w * s, w * kl, clipped ? w : 0.f, 0.f);
     return w * d;
 }
 
@@ -327,61 +468,184 @@ __global__ __launch_bounds__(256) void policy_terms_k(PolicyArgs a, const float*
     if (t >= a.rows) return;
     int lab;
     const bool valid = row_label(a.labels, t, a.ignore_index, a.vocab, lab);
-    const float w = valid ? policy_weight(a, t) : 0.f;
-    if ((threadIdx.x & 63) == 0) {
-        if (valid) a.coef[t] = policy_term(a, t, logp[t], w);
-        else { a.terms[t] = 0.f; a.terms[a.rows + t] = 0.f; a.terms[2 * a.rows + t] = 0.f; a.coef[t] = 0.f; }
-    }
+    int64_t s = 0, begin, end;
+    const bool inside = valid && policy_range(a, t, s, begin, end);
+    if ((threadIdx.x & 63) == 0) a.coef[t] = policy_term(a, t, (double)logp[t], policy_weight(a, inside, inside ? a.counts[s] : 0), a.terms[t]);
 }
 
-// forward and backward of one row: the coefficient needs nothing but the row itself
-template <bool BF, int NT>
+__device__ __forceinline__ void write_stats(const double* v, float kl_coef, float* stats) {
+    stats[0] = (float)(kl_coef > 0.f ? v[0] + (double)kl_coef * v[1] : v[0]);
+    stats[1] = (float)v[0];
+    stats[2] = (float)v[1];
+    stats[3] = (float)v[2];
+}
+
+// Counts, terms, coefficients and sums of a short batch in one workgroup: a launch less for each, which is all such a call costs.
+__global__ __launch_bounds__(1024) void policy_small_k(PolicyArgs a, const float* __restrict__ logp, float* __restrict__ stats) {
+    __shared__ int cnt[kSmallSeqs];
+    __shared__ double scratch[16];
+    constexpr int R = kSmallRows / 1024;
+    int seq[R];   // sequence of each of the thread's rows, -1: no label or outside
+    if (a.cu) {
+        for (int i = threadIdx.x; i < a.seqs; i += 1024) cnt[i] = 0;
+        __syncthreads();
+    }
+    int n = 0;
+#pragma unroll
+    for (int q = 0; q < R; ++q) {
+        const int64_t t = (int64_t)q * 1024 + threadIdx.x;
+        int lab;
+        seq[q] = t < a.rows && row_label(a.labels, t, a.ignore_index, a.vocab, lab) ? 0 : -1;
+        if (a.cu && seq[q] == 0) {
+            int lo = 0, hi = (int)a.seqs;   // how many of cu[1..S] are <= t
+            while (lo < hi) {
+                const int mid = (lo + hi) >> 1;
+                if ((int64_t)a.cu[mid + 1] <= t) lo = mid + 1; else hi = mid;
+            }
+            int64_t begin = 0, end = 0;
+            if (lo < (int)a.seqs) seq_range(a.cu, lo, a.rows, begin, end);
+            seq[q] = t >= begin && t < end ? lo : -1;
+            if (seq[q] >= 0) atomicAdd(&cnt[lo], 1);   // (whole numbers: the order does not matter)
+        }
+        n += seq[q] == 0;
+    }
+    if (a.cu) __syncthreads();
+    else n = (int)block_sum_d<16>((double)n, scratch);
+    double v[3] = {0.0, 0.0, 0.0};
+#pragma unroll
+    for (int q = 0; q < R; ++q) {
+        const int64_t t = (int64_t)q * 1024 + threadIdx.x;
+        if (t >= a.rows) continue;
+        float4 term = make_float4(0.f, 0.f, 0.f, 0.f);
+        a.coef[t] = seq[q] < 0 ? 0.f : policy_term(a, t, (double)logp[t], policy_weight(a, true, a.cu ? cnt[seq[q]] : n), term);
+        v[0] += (double)term.x; v[1] += (double)term.y; v[2] += (double)term.z;
+    }
+    for (int c = 0; c < 3; ++c) v[c] = block_sum_d<16>(v[c], scratch);
+    if (threadIdx.x == 0) write_stats(v, a.kl_coef, stats);
+}
+
+// Forward and backward of one row: its coefficient needs nothing but the row itself, so the logits are read once.  NV > 0: the row waits in registers, NV vectors a
+// thread; NV = 0 (longer rows): it is read again, from the last-level cache.
+template <bool BF, int NT, int NV, bool S>
 __global__ __launch_bounds__(NT) void policy_fused_k(PolicyArgs a, const void* logits, int64_t ld, void* dlogits, int64_t ldd, float* __restrict__ logp_out,
-                                                     float* __restrict__ lse_out, const float* __restrict__ dloss, float dloss_mul, float inv_tau) {
-    __shared__ float scratch[NT / 64];
+                                                     float* __restrict__ lse_out, const float* __restrict__ dloss, float dloss_mul, double inv_tau) {
+    typedef typename Elem<BF>::T T;
+    constexpr int N = Elem<BF>::N;
+    __shared__ float sh[NT / 32];
+    __shared__ int counted[NT / 64];
     __shared__ float coef_sh;
     const int64_t row = blockIdx.x;
-    typename Elem<BF>::T* d = (typename Elem<BF>::T*)dlogits + row * ldd;
+    const int vocab = a.vocab;
+    T* d = (T*)dlogits + row * ldd;
     int lab;
-    if (!row_label(a.labels, row, a.ignore_index, a.vocab, lab)) {
-        if (threadIdx.x == 0) {
-            logp_out[row] = 0.f; lse_out[row] = 0.f; a.coef[row] = 0.f;
-            a.terms[row] = 0.f; a.terms[a.rows + row] = 0.f; a.terms[2 * a.rows + row] = 0.f;
-        }
-        row_zero<BF, NT>(d, a.vocab);
+    if (!row_label(a.labels, row, a.ignore_index, vocab, lab)) {
+        if (threadIdx.x == 0) { logp_out[row] = 0.f; lse_out[row] = 0.f; a.coef[row] = 0.f; a.terms[row] = make_float4(0.f, 0.f, 0.f, 0.f); }
+        row_zero<BF, NT, S>(d, vocab);
         return;
     }
-    const typename Elem<BF>::T* x = (const typename Elem<BF>::T*)logits + row * ld;
-    const float k = inv_tau * kLog2e;
-    const RowStat st = row_stat<BF, NT>(x, a.vocab, k, scratch);
-    const float w = policy_weight(a, row);
+    // no counts (rows <= kCountRows NT): this workgroup's threads look at all labels, before the row's own loads
+    unsigned live = 0;
+    if (!a.counts) {
+#pragma unroll
+        for (int q = 0; q < kCountRows; ++q) {
+            const int64_t t = (int64_t)q * NT + threadIdx.x;
+            int other;
+            if (t < a.rows && row_label(a.labels, t, a.ignore_index, vocab, other)) live |= 1u << q;
+        }
+    }
+    const T* x = (const T*)logits + row * ld;
+    const float xl = Elem<BF>::get(x + lab);
+    const float k = (float)(inv_tau * kLog2e);
+    const int nv = vocab / N;
+    u32x4 v[NV > 0 ? NV : 1];
+    RowStat st;
+    if (NV > 0) {
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            const int i = threadIdx.x + j * NT;
+            v[j] = Elem<BF>::ninf();
+            if (i < nv) v[j] = ldv<S>(x + (int64_t)i * N);
+        }
+        float rest = -INFINITY;
+        if (nv * N + (int)threadIdx.x < vocab) rest = Elem<BF>::get(x + nv * N + threadIdx.x);
+        float m = rest;
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            float e[N];
+            Elem<BF>::unpack(v[j], e);
+#pragma unroll
+            for (int q = 0; q < N; ++q) m = fmaxf(m, e[q]);
+        }
+        // the vectors stay packed from pass to pass: kept unpacked they would not fit
+#pragma unroll
+        for (int j = 0; j < NV; ++j) asm volatile("" : "+v"(v[j]));
+        const float r = max_ref(m);
+        float s = exp2_((rest - r) * k);
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            float e[N];
+            Elem<BF>::unpack(v[j], e);
+#pragma unroll
+            for (int q = 0; q < N; ++q) s += exp2_((e[q] - r) * k);
+        }
+#pragma unroll
+        for (int j = 0; j < NV; ++j) asm volatile("" : "+v"(v[j]));
+        st = join_stats<NT>(m, s, k, sh);
+    } else {
+        st = row_stat<BF, NT, 4, false>(x, vocab, k, sh);
+    }
+    int64_t seq, begin, end;
+    const bool inside = policy_range(a, row, seq, begin, end);
+    int n = 0;
+    if (a.counts) {
+        n = inside ? a.counts[seq] : 0;
+    } else {
+#pragma unroll
+        for (int q = 0; q < kCountRows; ++q) {
+            const int64_t t = (int64_t)q * NT + threadIdx.x;
+            n += __popcll(__ballot((live >> q & 1u) && t >= begin && t < end));
+        }
+        if ((threadIdx.x & 63) == 0) counted[threadIdx.x >> 6] = n;
+        __syncthreads();
+        n = 0;
+#pragma unroll
+        for (int w = 0; w < NT / 64; ++w) n += counted[w];
+    }
     if (threadIdx.x == 0) {
-        const float logp = (Elem<BF>::get(x + lab) - st.m) * inv_tau - st.log_sum;
-        logp_out[row] = logp;
-        lse_out[row] = st.lse(inv_tau);
-        coef_sh = a.coef[row] = policy_term(a, row, logp, w);
+        const double logp = st.logp(xl, inv_tau);
+        logp_out[row] = (float)logp;
+        lse_out[row] = (float)st.lse(inv_tau);
+        coef_sh = a.coef[row] = policy_term(a, row, logp, policy_weight(a, inside, n), a.terms[row]);
     }
     __syncthreads();
-    const float g = coef_sh * dloss_mul * dloss[0] * inv_tau;
-    if (g == 0.f) row_zero<BF, NT>(d, a.vocab);
-    else row_grad<BF, NT>(x, d, a.vocab, k, st.m, g, g / st.s, lab);
+    const float g = coef_sh * dloss_mul * dloss[0] * (float)inv_tau;
+    if (g == 0.f) { row_zero<BF, NT, S>(d, vocab); return; }
+    const float g_p = g / st.s;
+    if (NV > 0) {
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            const int i = threadIdx.x + j * NT;
+            if (i < nv) stv<S>(d + (int64_t)i * N, grad_vector<BF>(v[j], k, st.m, g_p));
+        }
+        const int i = nv * N + threadIdx.x;
+        if (i < vocab) Elem<BF>::put(d + i, -g_p * exp2_((Elem<BF>::get(x + i) - st.m) * k));
+        if (owns<BF, NT>(lab, vocab)) Elem<BF>::put(d + lab, g - g_p * exp2_((xl - st.m) * k));
+    } else {
+        row_grad<BF, NT, 4, S>(x, d, vocab, k, st.m, g, g_p, lab, xl);
+    }
 }
 
 // stats = {loss, surrogate, KL, clipped share}
-__global__ __launch_bounds__(1024) void policy_stats_k(const float* __restrict__ terms, int64_t rows, float kl_coef, float* __restrict__ stats) {
+__global__ __launch_bounds__(1024) void policy_stats_k(const float4* __restrict__ terms, int64_t rows, float kl_coef, float* __restrict__ stats) {
     __shared__ double scratch[16];
-    double v[3];
-    for (int c = 0; c < 3; ++c) {
-        double s = 0.0;
-        for (int64_t t = threadIdx.x; t < rows; t += 1024) s += (double)terms[c * rows + t];
-        v[c] = block_sum_d<16>(s, scratch);
+    double v[3] = {0.0, 0.0, 0.0};
+#pragma unroll 8
+    for (int64_t t = threadIdx.x; t < rows; t += 1024) {
+        const float4 q = terms[t];
+        v[0] += (double)q.x; v[1] += (double)q.y; v[2] += (double)q.z;
     }
-    if (threadIdx.x == 0) {
-        stats[0] = (float)(kl_coef > 0.f ? v[0] + (double)kl_coef * v[1] : v[0]);
-        stats[1] = (float)v[0];
-        stats[2] = (float)v[1];
-        stats[3] = (float)v[2];
-    }
+    for (int c = 0; c < 3; ++c) v[c] = block_sum_d<16>(v[c], scratch);
+    if (threadIdx.x == 0) write_stats(v, kl_coef, stats);
 }
 
 constexpr int64_t kMaxVocab = int64_t(1) << 30;   // in-row indices are 32-bit
@@ -390,7 +654,7 @@ constexpr int64_t kMaxRows = 0x7fffffff;          // one workgroup per row
 #define IE_CHECK_LOGITS(fn)                                                                                                                              \
     IE_CHECK_ARG(dtype == IE_BF16 || dtype == IE_F32, fn ": bad dtype");                                                                                 \
     IE_CHECK_ARG(rows >= 0 && rows <= kMaxRows && vocab > 0 && vocab <= kMaxVocab && ld >= vocab, fn ": bad shape");                                     \
-    IE_CHECK_ARG(inv_temperature > 0.f && inv_temperature <= 3.0e38f, fn ": the temperature must be positive and finite")
+    IE_CHECK_ARG(inv_temperature >= 1e-30 && inv_temperature <= 1e30, fn ": the temperature must be positive and finite")
 
 // dlogits is either the logits (same address, same stride) or does not touch them
 bool overlap_ok(const void* x, int64_t ld, const void* d, int64_t ldd, int64_t rows, int64_t vocab, int dtype) {
@@ -400,38 +664,81 @@ bool overlap_ok(const void* x, int64_t ld, const void* d, int64_t ldd, int64_t r
     return xb + ((rows - 1) * ld + vocab) * es <= db || db + ((rows - 1) * ldd + vocab) * es <= xb;
 }
 
-int launch_logprob_fwd(const void* logits, int dtype, int64_t ld, const int64_t* labels, float* logp, float* lse, float* coef, int64_t rows, int64_t vocab,
-                       int64_t ignore_index, float inv_temperature, hipStream_t st) {
-    if (rows == 0) return IE_OK;
-    if (dtype == IE_BF16)
-        hipLaunchKernelGGL((logprob_fwd_k<true, 256>), dim3((unsigned)rows), dim3(256), 0, st, logits, ld, labels, logp, lse, coef, (int)vocab, ignore_index, inv_temperature);
-    else
-        hipLaunchKernelGGL((logprob_fwd_k<false, 256>), dim3((unsigned)rows), dim3(256), 0, st, logits, ld, labels, logp, lse, coef, (int)vocab, ignore_index, inv_temperature);
-    return ie_launch_status("log-probability launch");
+// logits beyond the 256 MB of the last-level cache stream past it
+bool streams(int64_t rows, int64_t vocab, int dtype) { return rows * vocab * (dtype == IE_BF16 ? 2 : 4) > (int64_t(256) << 20); }
+
+inline int vectors(int64_t vocab, int dtype) { return (int)(vocab / (dtype == IE_BF16 ? 8 : 4)); }
+
+struct Launch {
+    hipStream_t st;
+    int64_t rows;
+    template <int NT, typename F, typename... A> void go(F f, A... args) const { hipLaunchKernelGGL(f, dim3((unsigned)rows), dim3(NT), 0, st, args...); }
+};
+
+template <bool BF, bool S>
+void launch_fwd(const Launch& l, int nv, const void* logits, int64_t ld, const int64_t* labels, float* logp, float* lse, float* coef, int vocab, int64_t ignore_index, double inv_tau) {
+    if (nv <= 256) l.go<64>(logprob_fwd_k<BF, 64, S>, logits, ld, labels, logp, lse, coef, vocab, ignore_index, inv_tau);
+    else if (nv <= 2048) l.go<256>(logprob_fwd_k<BF, 256, S>, logits, ld, labels, logp, lse, coef, vocab, ignore_index, inv_tau);
+    else if (l.rows >= 512) l.go<512>(logprob_fwd_k<BF, 512, S>, logits, ld, labels, logp, lse, coef, vocab, ignore_index, inv_tau);
+    else l.go<1024>(logprob_fwd_k<BF, 1024, S>, logits, ld, labels, logp, lse, coef, vocab, ignore_index, inv_tau);
 }
+
+template <bool BF, bool S>
+void launch_bwd(const Launch& l, int nv, const void* logits, int64_t ld, void* dlogits, int64_t ldd, const int64_t* labels, const float* lse, const float* coef, const float* dloss,
+                float dloss_mul, int vocab, int64_t ignore_index, double inv_tau) {
+    if (nv <= 256) l.go<64>(logprob_bwd_k<BF, 64, 4, S>, logits, ld, dlogits, ldd, labels, lse, coef, dloss, dloss_mul, vocab, ignore_index, inv_tau);
+    else if (nv <= 2048) l.go<256>(logprob_bwd_k<BF, 256, 4, S>, logits, ld, dlogits, ldd, labels, lse, coef, dloss, dloss_mul, vocab, ignore_index, inv_tau);
+    else l.go<1024>(logprob_bwd_k<BF, 1024, 4, S>, logits, ld, dlogits, ldd, labels, lse, coef, dloss, dloss_mul, vocab, ignore_index, inv_tau);
+}
+
+// threads and vectors a thread of the fused kernel: the smallest that hold the row
+inline int fused_threads(int nv) { return nv <= 256 ? 64 : nv <= 2048 ? 256 : 1024; }
+
+template <bool BF, bool S>
+void launch_fused(const Launch& l, int nv, const PolicyArgs& a, const void* logits, int64_t ld, void* dlogits, int64_t ldd, float* logp, float* lse, const float* dloss, float dloss_mul,
+                  double inv_tau) {
+    if (nv <= 256) l.go<64>(policy_fused_k<BF, 64, 4, S>, a, logits, ld, dlogits, ldd, logp, lse, dloss, dloss_mul, inv_tau);
+    else if (nv <= 2048) l.go<256>(policy_fused_k<BF, 256, 8, S>, a, logits, ld, dlogits, ldd, logp, lse, dloss, dloss_mul, inv_tau);
+    else if (nv <= 4096) l.go<1024>(policy_fused_k<BF, 1024, 4, S>, a, logits, ld, dlogits, ldd, logp, lse, dloss, dloss_mul, inv_tau);
+    else if (nv <= 8192) l.go<1024>(policy_fused_k<BF, 1024, 8, S>, a, logits, ld, dlogits, ldd, logp, lse, dloss, dloss_mul, inv_tau);
+    else if (nv <= 12288) l.go<1024>(policy_fused_k<BF, 1024, 12, S>, a, logits, ld, dlogits, ldd, logp, lse, dloss, dloss_mul, inv_tau);
+    else if (nv <= 16384) l.go<1024>(policy_fused_k<BF, 1024, 16, S>, a, logits, ld, dlogits, ldd, logp, lse, dloss, dloss_mul, inv_tau);
+    else l.go<1024>(policy_fused_k<BF, 1024, 0, S>, a, logits, ld, dlogits, ldd, logp, lse, dloss, dloss_mul, inv_tau);
+}
+
+// fn<type, stream>(args...)
+#define IE_ROWS(fn, ...)                                                          \
+    do {                                                                          \
+        const bool s_ = streams(rows, vocab, dtype);                              \
+        const Launch l_ = {(hipStream_t)stream, rows};                            \
+        const int nv_ = vectors(vocab, dtype);                                    \
+        if (dtype == IE_BF16) {                                                   \
+            if (s_) fn<true, true>(l_, nv_, __VA_ARGS__);                         \
+            else fn<true, false>(l_, nv_, __VA_ARGS__);                           \
+        } else {                                                                  \
+            if (s_) fn<false, true>(l_, nv_, __VA_ARGS__);                        \
+            else fn<false, false>(l_, nv_, __VA_ARGS__);                          \
+        }                                                                         \
+    } while (0)
 
 }  // namespace
 
 extern "C" int ie_logprob_fwd(const void* logits, int dtype, int64_t ld, const int64_t* labels, float* logp, float* lse, int64_t rows, int64_t vocab,
-                              int64_t ignore_index, float inv_temperature, void* stream) {
+                              int64_t ignore_index, double inv_temperature, void* stream) {
     IE_CHECK_ARG(logits && labels && logp && lse, "ie_logprob_fwd: null pointer");
     IE_CHECK_LOGITS("ie_logprob_fwd");
-    return launch_logprob_fwd(logits, dtype, ld, labels, logp, lse, nullptr, rows, vocab, ignore_index, inv_temperature, (hipStream_t)stream);
+    if (rows == 0) return IE_OK;
+    IE_ROWS(launch_fwd, logits, ld, labels, logp, lse, (float*)nullptr, (int)vocab, ignore_index, inv_temperature);
+    return ie_launch_status("ie_logprob_fwd launch");
 }
 
 extern "C" int ie_logprob_bwd(const void* logits, int dtype, int64_t ld, void* dlogits, int64_t ldd, const int64_t* labels, const float* lse, const float* coef,
-                              const float* dloss, float dloss_mul, int64_t rows, int64_t vocab, int64_t ignore_index, float inv_temperature, void* stream) {
+                              const float* dloss, float dloss_mul, int64_t rows, int64_t vocab, int64_t ignore_index, double inv_temperature, void* stream) {
     IE_CHECK_ARG(logits && dlogits && labels && lse && coef, "ie_logprob_bwd: null pointer");
     IE_CHECK_LOGITS("ie_logprob_bwd");
     IE_CHECK_ARG(ldd >= vocab && overlap_ok(logits, ld, dlogits, ldd, rows, vocab, dtype), "ie_logprob_bwd: dlogits must be the logits themselves or lie apart from them");
     if (rows == 0) return IE_OK;
-    hipStream_t st = (hipStream_t)stream;
-    if (dtype == IE_BF16)
-        hipLaunchKernelGGL((logprob_bwd_k<true, 256>), dim3((unsigned)rows), dim3(256), 0, st, logits, ld, dlogits, ldd, labels, lse, coef, dloss, dloss_mul, (int)vocab,
-                           ignore_index, inv_temperature);
-    else
-        hipLaunchKernelGGL((logprob_bwd_k<false, 256>), dim3((unsigned)rows), dim3(256), 0, st, logits, ld, dlogits, ldd, labels, lse, coef, dloss, dloss_mul, (int)vocab,
-                           ignore_index, inv_temperature);
+    IE_ROWS(launch_bwd, logits, ld, dlogits, ldd, labels, lse, coef, dloss, dloss_mul, (int)vocab, ignore_index, inv_temperature);
     return ie_launch_status("ie_logprob_bwd launch");
 }
 
@@ -439,7 +746,7 @@ extern "C" int64_t ie_preference_loss_workspace(int64_t pairs) { return pairs > 
 
 extern "C" int ie_preference_loss_fwd(const void* logits, int dtype, int64_t ld, const int64_t* labels, const int32_t* cu_seqlens, const float* ref_logps, int kind,
                                       double beta, double label_smoothing, double margin, int average, float* loss, float* rewards, float* seq_logps, float* logp,
-                                      float* lse, float* coef, void* workspace, int64_t rows, int64_t vocab, int64_t pairs, int64_t ignore_index, float inv_temperature,
+                                      float* lse, float* coef, void* workspace, int64_t rows, int64_t vocab, int64_t pairs, int64_t ignore_index, double inv_temperature,
                                       void* stream) {
     IE_CHECK_ARG(logits && labels && cu_seqlens && loss && rewards && seq_logps && logp && lse && coef && workspace, "ie_preference_loss_fwd: null pointer");
     IE_CHECK_LOGITS("ie_preference_loss_fwd");
@@ -450,23 +757,27 @@ extern "C" int ie_preference_loss_fwd(const void* logits, int dtype, int64_t ld,
                  "ie_preference_loss_fwd: label smoothing lies in [0, 0.5] and belongs to the sigmoid form");
     IE_CHECK_ARG(margin >= -1e30 && margin <= 1e30 && (kind != IE_PREF_IPO || margin == 0.0), "ie_preference_loss_fwd: the squared form takes no margin");
     hipStream_t st = (hipStream_t)stream;
-    const int rc = launch_logprob_fwd(logits, dtype, ld, labels, logp, lse, coef, rows, vocab, ignore_index, inv_temperature, st);
-    if (rc != IE_OK) return rc;
+    if (rows > 0) IE_ROWS(launch_fwd, logits, ld, labels, logp, lse, coef, (int)vocab, ignore_index, inv_temperature);
     const PrefArgs a = {kind, average, beta, label_smoothing, margin};
-    hipLaunchKernelGGL(preference_pair_k, dim3((unsigned)pairs), dim3(256), 0, st, logp, labels, cu_seqlens, ref_logps, rows, pairs, ignore_index, (int)vocab, a,
-                       (double*)workspace, rewards, seq_logps, coef);
-    hipLaunchKernelGGL(preference_mean_k, dim3(1), dim3(256), 0, st, (const double*)workspace, pairs, loss);
+    const PrefRows r = {logp, labels, cu_seqlens, ref_logps, rows, pairs, ignore_index, (int)vocab, rewards, seq_logps, coef};
+    if (pairs <= kSmallPairs && rows <= kSmallRows) {
+        hipLaunchKernelGGL(preference_small_k, dim3(1), dim3(1024), 0, st, r, a, loss);
+    } else {
+        hipLaunchKernelGGL(preference_pair_k, dim3((unsigned)pairs), dim3(1024), 0, st, r, a, (double*)workspace);
+        hipLaunchKernelGGL(preference_mean_k, dim3(1), dim3(256), 0, st, (const double*)workspace, pairs, loss);
+    }
     return ie_launch_status("ie_preference_loss_fwd launch");
 }
 
-// terms [3][rows] floats, then the counts
-extern "C" int64_t ie_policy_loss_workspace(int64_t rows, int64_t seqs) { return rows < 0 || seqs < 0 ? 0 : (3 * rows + (seqs > 0 ? seqs : 1)) * 4; }
+// terms [rows] of four floats, then the counts
+extern "C" int64_t ie_policy_loss_workspace(int64_t rows, int64_t seqs) { return rows < 0 || seqs < 0 ? 0 : (4 * rows + (seqs > 0 ? seqs : 1)) * 4; }
 
 extern "C" int ie_policy_loss(const void* logits, int dtype, int64_t ld, void* dlogits, int64_t ldd, const int64_t* labels, const float* old_logps, const float* advantages,
                               const float* ref_logps, const int32_t* cu_seqlens, int64_t seqs, float clip_low, float clip_high, float kl_coef, const float* dloss,
                               float dloss_mul, float* stats, float* logp, float* lse, float* coef, void* workspace, int64_t rows, int64_t vocab, int64_t ignore_index,
-                              float inv_temperature, void* stream) {
+                              double inv_temperature, void* stream) {
     IE_CHECK_ARG(logits && labels && old_logps && advantages && stats && logp && lse && coef && workspace, "ie_policy_loss: null pointer");
+    IE_CHECK_ARG(((uintptr_t)workspace & 15) == 0, "ie_policy_loss: the workspace must be 16-byte aligned");
     IE_CHECK_LOGITS("ie_policy_loss");
     IE_CHECK_ARG((dlogits != nullptr) == (dloss != nullptr), "ie_policy_loss: dlogits and dloss come together");
     IE_CHECK_ARG(!dlogits || (ldd >= vocab && overlap_ok(logits, ld, dlogits, ldd, rows, vocab, dtype)),
@@ -475,22 +786,25 @@ extern "C" int ie_policy_loss(const void* logits, int dtype, int64_t ld, void* d
     IE_CHECK_ARG(clip_low >= 0.f && clip_low <= 1.f && clip_high >= 0.f && clip_high <= 1e30f, "ie_policy_loss: clip range");
     IE_CHECK_ARG(kl_coef >= 0.f && kl_coef <= 1e30f && (ref_logps || kl_coef == 0.f), "ie_policy_loss: a KL term needs the reference log-probabilities");
     hipStream_t st = (hipStream_t)stream;
+    int32_t* counts = (int32_t*)((float*)workspace + 4 * rows);
     PolicyArgs a;
     a.labels = labels; a.cu = cu_seqlens; a.old_logps = old_logps; a.adv = advantages; a.ref = ref_logps;
-    a.terms = (float*)workspace; a.counts = (const int32_t*)((float*)workspace + 3 * rows);
+    a.counts = counts; a.terms = (float4*)workspace;
     a.coef = coef; a.rows = rows; a.seqs = seqs; a.ignore_index = ignore_index; a.vocab = (int)vocab;
     a.low = clip_low; a.high = clip_high; a.kl_coef = kl_coef;
-    hipLaunchKernelGGL(policy_counts_k, dim3((unsigned)(cu_seqlens ? seqs : 1)), dim3(1024), 0, st, a, (int32_t*)((float*)workspace + 3 * rows));
+    if (!dlogits && rows <= kSmallRows && seqs <= kSmallSeqs) {
+        if (rows > 0) IE_ROWS(launch_fwd, logits, ld, labels, logp, lse, (float*)nullptr, (int)vocab, ignore_index, inv_temperature);
+        hipLaunchKernelGGL(policy_small_k, dim3(1), dim3(1024), 0, st, a, (const float*)logp, stats);
+        return ie_launch_status("ie_policy_loss launch");
+    }
+    if (dlogits && rows <= (int64_t)kCountRows * fused_threads(vectors(vocab, dtype))) a.counts = nullptr;
+    else hipLaunchKernelGGL(policy_counts_k, dim3((unsigned)(cu_seqlens ? seqs : 1)), dim3(1024), 0, st, a, counts);
     if (rows > 0 && dlogits) {
-        if (dtype == IE_BF16)
-            hipLaunchKernelGGL((policy_fused_k<true, 256>), dim3((unsigned)rows), dim3(256), 0, st, a, logits, ld, dlogits, ldd, logp, lse, dloss, dloss_mul, inv_temperature);
-        else
-            hipLaunchKernelGGL((policy_fused_k<false, 256>), dim3((unsigned)rows), dim3(256), 0, st, a, logits, ld, dlogits, ldd, logp, lse, dloss, dloss_mul, inv_temperature);
+        IE_ROWS(launch_fused, a, logits, ld, dlogits, ldd, logp, lse, dloss, dloss_mul, inv_temperature);
     } else if (rows > 0) {
-        const int rc = launch_logprob_fwd(logits, dtype, ld, labels, logp, lse, nullptr, rows, vocab, ignore_index, inv_temperature, st);
-        if (rc != IE_OK) return rc;
+        IE_ROWS(launch_fwd, logits, ld, labels, logp, lse, (float*)nullptr, (int)vocab, ignore_index, inv_temperature);
         hipLaunchKernelGGL(policy_terms_k, dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, a, (const float*)logp);
     }
-    hipLaunchKernelGGL(policy_stats_k, dim3(1), dim3(1024), 0, st, (const float*)workspace, rows, kl_coef, stats);
+    hipLaunchKernelGGL(policy_stats_k, dim3(1), dim3(1024), 0, st, (const float4*)workspace, rows, kl_coef, stats);
     return ie_launch_status("ie_policy_loss launch");
 }

@@ -1,4 +1,7 @@
-// L2 norm over a list of gradient tensors, and the clipped gradients.  The list travels as launch arguments, a fixed number of tensors a launch.
+// L2 norm over a list of gradient tensors, and the clipped gradients.
+//   norm = sqrt(sum_i g_i^2),  g_i <- g_i min(1, max_norm / (norm + 1e-6))
+// The list travels as launch arguments (4 KB of them: 192 tensors a launch of the norm, 136 of the clip), so that nothing is copied to the device first and a captured
+// graph holds all it needs.  Every tensor is cut into chunks; a workgroup finds its chunk's tensor in the launch's table.
 // HBM-bound: the norm reads every gradient once, the clip reads it again and writes it.
 #include "ie_common.h"
 
@@ -14,21 +17,29 @@ typedef u32x4 u32x4_any __attribute__((aligned(2)));   // 16 bytes at any elemen
 typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 typedef u32x2 u32x2_any __attribute__((aligned(2)));
 
-constexpr int kTensors = 96;                     // per launch: 96 x 28 bytes of arguments, well inside the 4 KB a launch carries
-constexpr int64_t kChunk = 1 << 15;              // elements a workgroup takes at a time
-constexpr int kNormBlocks = 2048;
+constexpr int kNormTensors = 192, kClipTensors = 136;
+constexpr int kNormBlocks = 2048;                // 8 workgroups of 256 threads a CU: one round of the chip
+constexpr int kJoined = 1024;                    // up to this many partial sums every clip workgroup adds them up itself: a launch less
+constexpr int kMinShift = 11, kMaxShift = 15;    // chunks of 2048 (one 8-element step of every thread) to 32768 elements
+constexpr int64_t kBf = int64_t(1) << 62, kOutBf = int64_t(1) << 61, kLen = kOutBf - 1;
 
-struct TensorList {
-    const void* in[kTensors];
-    void* out[kTensors];
-    int64_t numel[kTensors];
-    int first[kTensors + 1];                     // first chunk of tensor i; first[n] = all chunks
-    unsigned char in_bf[kTensors], out_bf[kTensors];
-    int n;
+struct NormList {
+    const void* in[kNormTensors];
+    int64_t len[kNormTensors];                   // elements, | kBf
+    int first[kNormTensors + 1];                 // first chunk of tensor i; first[n] = all chunks
+    int n, shift;
+};
+struct ClipList {
+    const void* in[kClipTensors];
+    void* out[kClipTensors];
+    int64_t len[kClipTensors];                   // elements, | kBf | kOutBf
+    int first[kClipTensors + 1];
+    int n, shift;
 };
 
-// tensor that chunk c belongs to (first[] is sorted; tensors without elements own no chunk)
-__device__ __forceinline__ int find_tensor(const TensorList& l, int c) {
+// tensor that chunk c belongs to (first[] grows strictly: tensors without elements are not in the table)
+template <typename L>
+__device__ __forceinline__ int find_tensor(const L& l, int c) {
     int lo = 0, hi = l.n;
     while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
@@ -37,35 +48,51 @@ __device__ __forceinline__ int find_tensor(const TensorList& l, int c) {
     return lo;
 }
 
-// Squares in 64 bits: a bf16 or fp32 product is exact there, and no gradient that fits its type overflows.
-__global__ __launch_bounds__(256) void grad_norm_k(TensorList l, double* __restrict__ partial) {
+template <bool S> __device__ __forceinline__ u32x4 ldv(const void* p) { return S ? __builtin_nontemporal_load((const u32x4_any*)p) : *(const u32x4_any*)p; }
+template <bool S> __device__ __forceinline__ void stv(void* p, const u32x4& v) {
+    if (S) __builtin_nontemporal_store(v, (u32x4_any*)p);
+    else *(u32x4_any*)p = v;
+}
+
+// Squares in 64 bits: the product of two bf16 or fp32 values is exact there, and no gradient that fits its type overflows.
+__device__ __forceinline__ void add_square(float x, double& acc) { acc = fma((double)x, (double)x, acc); }
+
+template <bool BF, bool S>
+__device__ __forceinline__ void chunk_squares(const void* in, int64_t base, int n, double& acc) {
+    constexpr int N = BF ? 8 : 4, U = 4;
+    const char* p = (const char*)in + base * (BF ? 2 : 4);
+    auto add = [&](const u32x4& v) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            if (BF) { add_square(bflo(v[e]), acc); add_square(bfhi(v[e]), acc); }
+            else add_square(__uint_as_float(v[e]), acc);
+        }
+    };
+    const int nv = n / N;
+    int i = threadIdx.x;
+    for (; i + (U - 1) * 256 < nv; i += U * 256) {
+        u32x4 w[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) w[u] = ldv<S>(p + (int64_t)(i + u * 256) * 16);
+#pragma unroll
+        for (int u = 0; u < U; ++u) add(w[u]);
+    }
+    for (; i < nv; i += 256) add(ldv<S>(p + (int64_t)i * 16));
+    if (nv * N + (int)threadIdx.x < n) add_square(BF ? bf2f(((const bf16_t*)p)[nv * N + threadIdx.x]) : ((const float*)p)[nv * N + threadIdx.x], acc);
+}
+
+template <bool S>
+__global__ __launch_bounds__(256) void grad_norm_k(NormList l, double* __restrict__ partial) {
     __shared__ double scratch[4];
     double acc = 0.0;
-    for (int c = blockIdx.x; c < l.first[l.n]; c += gridDim.x) {
-        const int t = find_tensor(l, c);
-        const int64_t base = (int64_t)(c - l.first[t]) * kChunk;
-        const int n = (int)min(l.numel[t] - base, kChunk);
-        if (l.in_bf[t]) {
-            const bf16_t* p = (const bf16_t*)l.in[t] + base;
-            for (int i = threadIdx.x; i < n / 8; i += 256) {
-                const u32x4 v = *(const u32x4_any*)(p + i * 8);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const double a = (double)bflo(v[e]), b = (double)bfhi(v[e]);
-                    acc = fma(a, a, acc);
-                    acc = fma(b, b, acc);
-                }
-            }
-            for (int i = n / 8 * 8 + threadIdx.x; i < n; i += 256) { const double a = (double)bf2f(p[i]); acc = fma(a, a, acc); }
-        } else {
-            const float* p = (const float*)l.in[t] + base;
-            for (int i = threadIdx.x; i < n / 4; i += 256) {
-                const u32x4 v = *(const u32x4_any*)(p + i * 4);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) { const double a = (double)__uint_as_float(v[e]); acc = fma(a, a, acc); }
-            }
-            for (int i = n / 4 * 4 + threadIdx.x; i < n; i += 256) { const double a = (double)p[i]; acc = fma(a, a, acc); }
-        }
+    const int total = l.first[l.n];
+    int t = find_tensor(l, blockIdx.x);
+    for (int c = blockIdx.x; c < total; c += gridDim.x) {
+        while (l.first[t + 1] <= c) ++t;
+        const int64_t base = (int64_t)(c - l.first[t]) << l.shift, len = l.len[t];
+        const int n = (int)min((len & kLen) - base, (int64_t)1 << l.shift);
+        if (len & kBf) chunk_squares<true, S>(l.in[t], base, n, acc);
+        else chunk_squares<false, S>(l.in[t], base, n, acc);
     }
     acc = wave_sum_d(acc);
     if ((threadIdx.x & 63) == 0) scratch[threadIdx.x >> 6] = acc;
@@ -73,145 +100,212 @@ __global__ __launch_bounds__(256) void grad_norm_k(TensorList l, double* __restr
     if (threadIdx.x == 0) partial[blockIdx.x] = scratch[0] + scratch[1] + scratch[2] + scratch[3];
 }
 
-__global__ __launch_bounds__(256) void grad_norm_finish_k(const double* __restrict__ partial, int64_t n, float* __restrict__ norm) {
-    __shared__ double scratch[4];
+// norm from the partial sums, in a fixed order; every thread returns it
+__device__ __forceinline__ float join_norm(const double* __restrict__ partial, int n, double* scratch) {
     double acc = 0.0;
-    for (int64_t i = threadIdx.x; i < n; i += 256) acc += partial[i];
+#pragma unroll 4
+    for (int i = threadIdx.x; i < n; i += 256) acc += partial[i];
     acc = wave_sum_d(acc);
     if ((threadIdx.x & 63) == 0) scratch[threadIdx.x >> 6] = acc;
     __syncthreads();
-    if (threadIdx.x == 0) norm[0] = (float)sqrt(scratch[0] + scratch[1] + scratch[2] + scratch[3]);
+    return (float)sqrt(scratch[0] + scratch[1] + scratch[2] + scratch[3]);
 }
 
-__global__ __launch_bounds__(256) void grad_clip_k(TensorList l, const float* __restrict__ norm, double max_norm, int in_place) {
-    const double q = max_norm / ((double)norm[0] + 1e-6);
-    const float f = q < 1.0 ? (float)q : q == q ? 1.f : (float)q;
+__global__ __launch_bounds__(256) void grad_norm_finish_k(const double* __restrict__ partial, int n, float* __restrict__ norm) {
+    __shared__ double scratch[4];
+    const float v = join_norm(partial, n, scratch);
+    if (threadIdx.x == 0) norm[0] = v;
+}
+
+// N elements at element i of a tensor: the step of one thread.  Its store is never wider than 16 bytes, so that a wave's stores lie side by side (8 fp32 values a
+// thread, two stores 32 bytes apart, took 1673 us where this takes 1223: 0.87e9 bf16 gradients into fp32).
+template <bool BF, int N, bool S> struct Step;
+template <bool S> struct Step<true, 8, S> {
+    u32x4 v;
+    __device__ __forceinline__ void load(const bf16_t* p) { v = ldv<S>(p); }
+    __device__ __forceinline__ void unpack(float* f) const {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) { f[2 * e] = bflo(v[e]); f[2 * e + 1] = bfhi(v[e]); }
+    }
+    __device__ __forceinline__ static void store(bf16_t* p, const float* f) {
+        u32x4 w;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[e] = pack2bf(f[2 * e], f[2 * e + 1]);
+        stv<S>(p, w);
+    }
+};
+template <bool S> struct Step<true, 4, S> {
+    u32x2 v;
+    __device__ __forceinline__ void load(const bf16_t* p) { v = S ? __builtin_nontemporal_load((const u32x2_any*)p) : *(const u32x2_any*)p; }
+    __device__ __forceinline__ void unpack(float* f) const { f[0] = bflo(v[0]); f[1] = bfhi(v[0]); f[2] = bflo(v[1]); f[3] = bfhi(v[1]); }
+    __device__ __forceinline__ static void store(bf16_t* p, const float* f) {
+        const u32x2 w = {pack2bf(f[0], f[1]), pack2bf(f[2], f[3])};
+        if (S) __builtin_nontemporal_store(w, (u32x2_any*)p);
+        else *(u32x2_any*)p = w;
+    }
+};
+template <bool S> struct Step<false, 4, S> {
+    u32x4 v;
+    __device__ __forceinline__ void load(const float* p) { v = ldv<S>(p); }
+    __device__ __forceinline__ void unpack(float* f) const {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) f[e] = __uint_as_float(v[e]);
+    }
+    __device__ __forceinline__ static void store(float* p, const float* f) {
+        const u32x4 w = {__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3])};
+        stv<S>(p, w);
+    }
+};
+template <bool BF> struct Type;
+template <> struct Type<true> {
+    typedef bf16_t T;
+    static __device__ __forceinline__ float get(T x) { return bf2f(x); }
+    static __device__ __forceinline__ T put(float x) { return f2bf(x); }
+};
+template <> struct Type<false> {
+    typedef float T;
+    static __device__ __forceinline__ float get(T x) { return x; }
+    static __device__ __forceinline__ T put(float x) { return x; }
+};
+
+template <bool IB, bool OB, bool S>
+__device__ __forceinline__ void chunk_scale(const void* in, void* out, int64_t base, int n, float f) {
+    constexpr int N = IB && OB ? 8 : 4, U = 4;
+    const typename Type<IB>::T* p = (const typename Type<IB>::T*)in + base;
+    typename Type<OB>::T* o = (typename Type<OB>::T*)out + base;
+    const int ns = n / N;
+    auto scale = [&](const Step<IB, N, S>& q, int i) {
+        float v[N];
+        q.unpack(v);
+#pragma unroll
+        for (int e = 0; e < N; ++e) v[e] *= f;
+        Step<OB, N, S>::store(o + i * N, v);
+    };
+    int i = threadIdx.x;
+    for (; i + (U - 1) * 256 < ns; i += U * 256) {
+        Step<IB, N, S> q[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) q[u].load(p + (i + u * 256) * N);
+#pragma unroll
+        for (int u = 0; u < U; ++u) scale(q[u], i + u * 256);
+    }
+    for (; i < ns; i += 256) {
+        Step<IB, N, S> q;
+        q.load(p + i * N);
+        scale(q, i);
+    }
+    i = ns * N + threadIdx.x;
+    if (i < n) o[i] = Type<OB>::put(Type<IB>::get(p[i]) * f);
+}
+
+// partial sums given: the norm is added up here (and kept by the first workgroup if norm_out is given); otherwise norm holds it
+template <bool S>
+__global__ __launch_bounds__(256) void grad_clip_k(ClipList l, const double* __restrict__ partial, int parts, const float* norm, float* norm_out, double max_norm, int in_place) {
+    __shared__ double scratch[4];
+    const float nrm = partial ? join_norm(partial, parts, scratch) : norm[0];
+    if (norm_out && blockIdx.x == 0 && threadIdx.x == 0) norm_out[0] = nrm;
+    const double q = max_norm / ((double)nrm + 1e-6);
+    const float f = q >= 1.0 ? 1.f : (float)q;   // (NaN stays NaN)
     if (in_place && f == 1.f) return;
     const int c = blockIdx.x, t = find_tensor(l, c);
-    const int64_t base = (int64_t)(c - l.first[t]) * kChunk;
-    const int n = (int)min(l.numel[t] - base, kChunk);
-    if (l.in_bf[t]) {
-        const bf16_t* p = (const bf16_t*)l.in[t] + base;
-        if (l.out_bf[t]) {
-            bf16_t* o = (bf16_t*)l.out[t] + base;
-            for (int i = threadIdx.x; i < n / 8; i += 256) {
-                u32x4 v = *(const u32x4_any*)(p + i * 8);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] = pack2bf(bflo(v[e]) * f, bfhi(v[e]) * f);
-                *(u32x4_any*)(o + i * 8) = v;
-            }
-            for (int i = n / 8 * 8 + threadIdx.x; i < n; i += 256) o[i] = f2bf(bf2f(p[i]) * f);
-        } else {
-            float* o = (float*)l.out[t] + base;
-            for (int i = threadIdx.x; i < n / 4; i += 256) {   // 4 elements a thread: the stores are 16 bytes
-                const u32x2 v = *(const u32x2_any*)(p + i * 4);
-                u32x4 w;
-                w[0] = __float_as_uint(bflo(v[0]) * f); w[1] = __float_as_uint(bfhi(v[0]) * f);
-                w[2] = __float_as_uint(bflo(v[1]) * f); w[3] = __float_as_uint(bfhi(v[1]) * f);
-                *(u32x4_any*)(o + i * 4) = w;
-            }
-            for (int i = n / 4 * 4 + threadIdx.x; i < n; i += 256) o[i] = bf2f(p[i]) * f;
-        }
+    const int64_t base = (int64_t)(c - l.first[t]) << l.shift, len = l.len[t];
+    const int n = (int)min((len & kLen) - base, (int64_t)1 << l.shift);
+    if (len & kBf) {
+        if (len & kOutBf) chunk_scale<true, true, S>(l.in[t], l.out[t], base, n, f);
+        else chunk_scale<true, false, S>(l.in[t], l.out[t], base, n, f);
     } else {
-        const float* p = (const float*)l.in[t] + base;
-        if (l.out_bf[t]) {
-            bf16_t* o = (bf16_t*)l.out[t] + base;
-            for (int i = threadIdx.x; i < n / 4; i += 256) {
-                const u32x4 v = *(const u32x4_any*)(p + i * 4);
-                u32x2 w;
-                w[0] = pack2bf(__uint_as_float(v[0]) * f, __uint_as_float(v[1]) * f);
-                w[1] = pack2bf(__uint_as_float(v[2]) * f, __uint_as_float(v[3]) * f);
-                *(u32x2_any*)(o + i * 4) = w;
-            }
-            for (int i = n / 4 * 4 + threadIdx.x; i < n; i += 256) o[i] = f2bf(p[i] * f);
-        } else {
-            float* o = (float*)l.out[t] + base;
-            for (int i = threadIdx.x; i < n / 4; i += 256) {
-                u32x4 v = *(const u32x4_any*)(p + i * 4);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * f);
-                *(u32x4_any*)(o + i * 4) = v;
-            }
-            for (int i = n / 4 * 4 + threadIdx.x; i < n; i += 256) o[i] = p[i] * f;
-        }
+        if (len & kOutBf) chunk_scale<false, true, S>(l.in[t], l.out[t], base, n, f);
+        else chunk_scale<false, false, S>(l.in[t], l.out[t], base, n, f);
     }
-}
-
-int check_list(const char* fn, const void* const* ptrs, const int64_t* numels, const int* dtypes, int64_t n) {
-    if (n < 0 || n > (int64_t(1) << 24) || (n > 0 && (!ptrs || !numels || !dtypes))) { ie_set_error(fn); return IE_ERR_INVALID; }
-    for (int64_t i = 0; i < n; ++i)
-        if (numels[i] < 0 || numels[i] > (int64_t(1) << 40) || (numels[i] > 0 && !ptrs[i]) || (dtypes[i] != IE_BF16 && dtypes[i] != IE_F32)) { ie_set_error(fn); return IE_ERR_INVALID; }
-    return IE_OK;
 }
 
 inline int64_t esize(int dtype) { return dtype == IE_BF16 ? 2 : 4; }
-inline int64_t chunks(int64_t numel) { return (numel + kChunk - 1) / kChunk; }
 
-// the next launch's tensors, starting at i: at most kTensors of them and fewer than 2^30 chunks in all
-int64_t fill(TensorList& l, int64_t i, const void* const* ptrs, const int64_t* numels, const int* dtypes, void* const* outs, const int* out_dtypes, int64_t n) {
-    l.n = 0;
-    int64_t total = 0;
-    for (; i < n && l.n < kTensors; ++i) {
-        if (numels[i] == 0) continue;
-        if (total + chunks(numels[i]) > (int64_t(1) << 30)) break;
-        l.in[l.n] = ptrs[i];
-        l.out[l.n] = outs ? outs[i] : (void*)ptrs[i];
-        l.numel[l.n] = numels[i];
-        l.in_bf[l.n] = dtypes[i] == IE_BF16;
-        l.out_bf[l.n] = outs ? out_dtypes[i] == IE_BF16 : l.in_bf[l.n];
-        l.first[l.n++] = (int)total;
-        total += chunks(numels[i]);
+struct Lists {
+    const void* const* ptrs;
+    const int64_t* numels;
+    const int* dtypes;
+    void* const* outs;
+    const int* out_dtypes;
+    int64_t n, elems, bytes;
+    int shift;
+    bool stream;   // beyond the 256 MB of the last-level cache: past it
+};
+
+int check_list(const char* msg, Lists& l) {
+    if (l.n < 0 || l.n > (int64_t(1) << 24) || (l.n > 0 && (!l.ptrs || !l.numels || !l.dtypes))) { ie_set_error(msg); return IE_ERR_INVALID; }
+    l.elems = l.bytes = 0;
+    for (int64_t i = 0; i < l.n; ++i) {
+        if (l.numels[i] < 0 || l.numels[i] > (int64_t(1) << 38) || (l.numels[i] > 0 && !l.ptrs[i]) || (l.dtypes[i] != IE_BF16 && l.dtypes[i] != IE_F32)) {
+            ie_set_error(msg);
+            return IE_ERR_INVALID;
+        }
+        l.elems += l.numels[i];
+        l.bytes += l.numels[i] * esize(l.dtypes[i]);
     }
-    l.first[l.n] = (int)total;
+    // 4096 chunks or more, where the list is long enough for it
+    l.shift = kMinShift;
+    while (l.shift < kMaxShift && (l.elems >> l.shift) > 4096) ++l.shift;
+    l.stream = l.bytes > (int64_t(256) << 20);
+    return IE_OK;
+}
+
+inline void put_out(NormList&, int, const Lists&, int64_t) {}
+inline void put_out(ClipList& t, int k, const Lists& l, int64_t i) {
+    t.out[k] = l.outs ? l.outs[i] : (void*)l.ptrs[i];
+    if ((l.outs ? l.out_dtypes[i] : l.dtypes[i]) == IE_BF16) t.len[k] |= kOutBf;
+}
+
+// the next launch's tensors, from i on; returns where the one after it starts.  (2^38 elements are 2^23 chunks at the largest chunk: one tensor always fits.)
+template <int CAP, typename L>
+int64_t fill(L& t, int64_t i, const Lists& l) {
+    t.n = 0;
+    t.shift = l.shift;
+    int64_t total = 0;
+    for (; i < l.n && t.n < CAP; ++i) {
+        if (l.numels[i] == 0) continue;
+        const int64_t chunks = (l.numels[i] + (int64_t(1) << l.shift) - 1) >> l.shift;
+        if (total + chunks > (int64_t(1) << 30)) break;
+        t.in[t.n] = l.ptrs[i];
+        t.len[t.n] = l.numels[i] | (l.dtypes[i] == IE_BF16 ? kBf : 0);
+        put_out(t, t.n, l, i);
+        t.first[t.n++] = (int)total;
+        total += chunks;
+    }
+    t.first[t.n] = (int)total;
     return i;
 }
 
-inline int norm_blocks(const TensorList& l) { return std::min(l.first[l.n], kNormBlocks); }
-
-}  // namespace
-
-// launches of kTensors tensors each (one tensor at least), kNormBlocks partial sums each
-extern "C" int64_t ie_grad_norm_workspace(int64_t n) { return n < 0 ? 0 : (n / kTensors + 1) * kNormBlocks * 8; }
-
-extern "C" int ie_grad_norm(const void* const* ptrs, const int64_t* numels, const int* dtypes, int64_t n, void* workspace, float* norm, void* stream) {
-    IE_CHECK_ARG(workspace && norm, "ie_grad_norm: null pointer");
-    const int rc = check_list("ie_grad_norm: bad tensor list", ptrs, numels, dtypes, n);
-    if (rc != IE_OK) return rc;
-    hipStream_t st = (hipStream_t)stream;
-    TensorList l;
-    int64_t used = 0;
-    for (int64_t i = 0; i < n;) {
-        i = fill(l, i, ptrs, numels, dtypes, nullptr, nullptr, n);
-        if (l.n == 0) continue;
-        const int blocks = norm_blocks(l);
-        hipLaunchKernelGGL(grad_norm_k, dim3((unsigned)blocks), dim3(256), 0, st, l, (double*)workspace + used);
+// partial sums of the whole list; returns how many
+int launch_norm(const Lists& l, double* partial, hipStream_t st) {
+    NormList t;
+    int used = 0;
+    for (int64_t i = 0; i < l.n;) {
+        i = fill<kNormTensors>(t, i, l);
+        if (t.n == 0) continue;
+        const int blocks = std::min(t.first[t.n], kNormBlocks);
+        if (l.stream) hipLaunchKernelGGL((grad_norm_k<true>), dim3((unsigned)blocks), dim3(256), 0, st, t, partial + used);
+        else hipLaunchKernelGGL((grad_norm_k<false>), dim3((unsigned)blocks), dim3(256), 0, st, t, partial + used);
         used += blocks;
     }
-    hipLaunchKernelGGL(grad_norm_finish_k, dim3(1), dim3(256), 0, st, (const double*)workspace, used, norm);
-    return ie_launch_status("ie_grad_norm launch");
+    return used;
 }
 
-extern "C" int ie_grad_clip(const void* const* ptrs, const int64_t* numels, const int* dtypes, void* const* outs, const int* out_dtypes, int64_t n,
-                            const float* norm, double max_norm, void* stream) {
-    IE_CHECK_ARG(norm, "ie_grad_clip: null pointer");
-    IE_CHECK_ARG(max_norm >= 0.0, "ie_grad_clip: max_norm must not be negative");
-    const int rc = check_list("ie_grad_clip: bad tensor list", ptrs, numels, dtypes, n);
-    if (rc != IE_OK) return rc;
-    IE_CHECK_ARG(!outs || out_dtypes || n == 0, "ie_grad_clip: null pointer");
-    // every written range is disjoint from every other range, except from the one it is made of (same address, same type)
-    struct Range { const char *a, *b; int64_t owner; bool written; };
+// every written range is disjoint from every other range, except from the one it is made of (same address, same type)
+int check_overlap(const Lists& l) {
+    struct Range { const char *a, *b; bool written; };
     std::vector<Range> rs;
     try {
-        rs.reserve((size_t)n * 2);
-        for (int64_t i = 0; i < n; ++i) {
-            if (numels[i] == 0) continue;
-            const char* p = (const char*)ptrs[i];
-            const bool same = !outs || (outs[i] == ptrs[i] && out_dtypes[i] == dtypes[i]);
-            rs.push_back({p, p + numels[i] * esize(dtypes[i]), i, same});
+        rs.reserve((size_t)l.n * 2);
+        for (int64_t i = 0; i < l.n; ++i) {
+            if (l.numels[i] == 0) continue;
+            const char* p = (const char*)l.ptrs[i];
+            const bool same = !l.outs || (l.outs[i] == l.ptrs[i] && l.out_dtypes[i] == l.dtypes[i]);
+            rs.push_back({p, p + l.numels[i] * esize(l.dtypes[i]), same});
             if (same) continue;
-            IE_CHECK_ARG(outs[i] && (out_dtypes[i] == IE_BF16 || out_dtypes[i] == IE_F32), "ie_grad_clip: bad output list");
-            const char* o = (const char*)outs[i];
-            rs.push_back({o, o + numels[i] * esize(out_dtypes[i]), i, true});
+            IE_CHECK_ARG(l.outs[i] && (l.out_dtypes[i] == IE_BF16 || l.out_dtypes[i] == IE_F32), "ie_grad_clip: bad output list");
+            const char* o = (const char*)l.outs[i];
+            rs.push_back({o, o + l.numels[i] * esize(l.out_dtypes[i]), true});
         }
         std::sort(rs.begin(), rs.end(), [](const Range& x, const Range& y) { return x.a < y.a; });
     } catch (...) {
@@ -224,12 +318,48 @@ extern "C" int ie_grad_clip(const void* const* ptrs, const int64_t* numels, cons
         end_any = std::max(end_any, r.b);
         if (r.written) end_written = std::max(end_written, r.b);
     }
+    return IE_OK;
+}
+
+}  // namespace
+
+extern "C" int64_t ie_grad_norm_workspace(int64_t n) { return n < 0 ? 0 : (n / kNormTensors + 1) * kNormBlocks * 8; }
+
+extern "C" int ie_grad_norm(const void* const* ptrs, const int64_t* numels, const int* dtypes, int64_t n, void* workspace, float* norm, void* stream) {
+    IE_CHECK_ARG(workspace && norm, "ie_grad_norm: null pointer");
+    Lists l = {ptrs, numels, dtypes, nullptr, nullptr, n, 0, 0, 0, false};
+    const int rc = check_list("ie_grad_norm: bad tensor list", l);
+    if (rc != IE_OK) return rc;
+    const int parts = launch_norm(l, (double*)workspace, (hipStream_t)stream);
+    hipLaunchKernelGGL(grad_norm_finish_k, dim3(1), dim3(256), 0, (hipStream_t)stream, (const double*)workspace, parts, norm);
+    return ie_launch_status("ie_grad_norm launch");
+}
+
+extern "C" int ie_grad_clip(const void* const* ptrs, const int64_t* numels, const int* dtypes, void* const* outs, const int* out_dtypes, int64_t n, double max_norm,
+                            void* workspace, float* norm, void* stream) {
+    IE_CHECK_ARG(workspace && norm, "ie_grad_clip: null pointer");
+    IE_CHECK_ARG(max_norm >= 0.0, "ie_grad_clip: max_norm must not be negative");
+    Lists l = {ptrs, numels, dtypes, outs, out_dtypes, n, 0, 0, 0, false};
+    int rc = check_list("ie_grad_clip: bad tensor list", l);
+    if (rc != IE_OK) return rc;
+    IE_CHECK_ARG(!outs || out_dtypes || n == 0, "ie_grad_clip: null pointer");
+    rc = check_overlap(l);
+    if (rc != IE_OK) return rc;
     hipStream_t st = (hipStream_t)stream;
-    TensorList l;
+    const double* partial = (const double*)workspace;
+    const int parts = launch_norm(l, (double*)workspace, st);
+    const bool joined = parts <= kJoined && parts > 0;
+    if (!joined) hipLaunchKernelGGL(grad_norm_finish_k, dim3(1), dim3(256), 0, st, partial, parts, norm);
+    ClipList t;
+    float* norm_out = joined ? norm : nullptr;
     for (int64_t i = 0; i < n;) {
-        i = fill(l, i, ptrs, numels, dtypes, outs, out_dtypes, n);
-        if (l.n == 0) continue;
-        hipLaunchKernelGGL(grad_clip_k, dim3((unsigned)l.first[l.n]), dim3(256), 0, st, l, norm, max_norm, (int)(outs == nullptr));
+        i = fill<kClipTensors>(t, i, l);
+        if (t.n == 0) continue;
+        const dim3 grid((unsigned)t.first[t.n]);
+        const double* from = joined ? partial : nullptr;
+        if (l.stream) hipLaunchKernelGGL((grad_clip_k<true>), grid, dim3(256), 0, st, t, from, parts, (const float*)norm, norm_out, max_norm, (int)(outs == nullptr));
+        else hipLaunchKernelGGL((grad_clip_k<false>), grid, dim3(256), 0, st, t, from, parts, (const float*)norm, norm_out, max_norm, (int)(outs == nullptr));
+        norm_out = nullptr;
     }
     return ie_launch_status("ie_grad_clip launch");
 }

@@ -6,9 +6,9 @@ device pointers + sizes + ``torch.cuda.current_stream().cuda_stream`` to libinte
 on a HIP device is a ``ValueError``.
 """
 import array
-import collections
 import ctypes
 import math
+import operator
 
 import torch
 
@@ -295,19 +295,59 @@ def ce_bwd(logits, labels, lse, dloss, count, dloss_mul=1.0, ignore_index=-100, 
 
 
 # ------------------------------------------------------------------------------------------ preference / policy losses
-PreferenceLoss = collections.namedtuple("PreferenceLoss", "loss rewards seq_logps logp lse coef")
-PolicyLoss = collections.namedtuple("PolicyLoss", "loss stats logp lse coef")
+class PreferenceLoss:
+    """What preference_loss_fwd found, fp32 on the device: loss [1], rewards [P, 2], seq_logps [2 P], and per row logp, lse, coef = d loss / d logp [rows].
+    (Each is cut out of its buffer when asked for: a view costs the host a microsecond, and a training step asks for few.)"""
+
+    __slots__ = ("_rows", "_small", "_seqs")
+
+    def __init__(self, rows, small, seqs):
+        self._rows, self._small, self._seqs = rows, small, seqs
+
+    loss = property(lambda self: self._small[2 * self._seqs:2 * self._seqs + 1])
+    rewards = property(lambda self: self._small[:self._seqs].view(-1, 2))
+    seq_logps = property(lambda self: self._small[self._seqs:2 * self._seqs])
+    logp = property(lambda self: self._rows[0])
+    lse = property(lambda self: self._rows[1])
+    coef = property(lambda self: self._rows[2])
+
+
+class PolicyLoss:
+    """What policy_loss_fwd / policy_loss_fwd_bwd found, fp32 on the device: stats [4] = loss, policy term, KL, clipped share; loss [1]; and per row logp, lse,
+    coef = d loss / d logp [rows]."""
+
+    __slots__ = ("_rows", "stats")
+
+    def __init__(self, rows, stats):
+        self._rows, self.stats = rows, stats
+
+    loss = property(lambda self: self.stats[:1])
+    logp = property(lambda self: self._rows[0])
+    lse = property(lambda self: self._rows[1])
+    coef = property(lambda self: self._rows[2])
+
+
 _PREFERENCE_KINDS = {"sigmoid": 0, "hinge": 1, "ipo": 2}
 
 
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)   # (a Stream object costs 3 us)
+
+
 def _on_current_device(*tensors):
-    """The kernels run on the current device's current stream: a tensor elsewhere is refused, not fetched."""
-    dev = tensors[0].device
+    """Index of the one device all tensors are on.  The kernels run on the current device's current stream: a tensor elsewhere is refused, not fetched."""
+    index = tensors[0].get_device()
     for t in tensors:
-        if t is not None and t.device != dev:
-            raise ValueError(f"tensors on {dev} and {t.device} in one call")
-    if dev.type == "cuda" and dev.index != torch.cuda.current_device():
-        raise ValueError(f"tensors on {dev}, current device cuda:{torch.cuda.current_device()}: switch with torch.cuda.device")
+        if t is not None and t.get_device() != index:
+            raise ValueError(f"tensors on {tensors[0].device} and {t.device} in one call")
+    if index < 0:
+        raise ValueError("internevo_amd kernels need HIP device tensors (no CPU fallback)")
+    if index != torch.cuda.current_device():
+        raise ValueError(f"tensors on cuda:{index}, current device cuda:{torch.cuda.current_device()}: switch with torch.cuda.device")
+    return index
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr() or _p(t).value
 
 
 def _logit_rows(logits, name="logits"):
@@ -321,7 +361,7 @@ def _logit_rows(logits, name="logits"):
 
 
 def _row_vector(t, rows, dtype, name):
-    if t.shape != (rows,) or t.dtype != dtype or not t.is_contiguous():
+    if t.dtype != dtype or t.dim() != 1 or t.numel() != rows or not t.is_contiguous():
         raise ValueError(f"{name}: expected a contiguous {dtype} tensor of shape ({rows},), got {t.dtype} {tuple(t.shape)}")
 
 
@@ -336,7 +376,7 @@ def _inv_temperature(temperature):
     return 1.0 / temperature
 
 
-def _dlogits_for(logits, dlogits, rows, vocab):
+def _dlogits_for(logits, dlogits):
     if dlogits is None:
         dlogits = logits
     if dlogits.shape != logits.shape or dlogits.dtype != logits.dtype:
@@ -351,29 +391,44 @@ def token_logprobs(logits, labels, ignore_index=-100, temperature=1.0):
     _row_vector(labels, rows, torch.int64, "labels")
     inv = _inv_temperature(temperature)
     dt = _dt(logits)
-    _on_current_device(logits, labels)
+    stream = _raw_stream(_on_current_device(logits, labels))
     logp = torch.empty(rows, dtype=torch.float32, device=logits.device)
-    lse = torch.empty(rows, dtype=torch.float32, device=logits.device)
-    check(_L().ie_logprob_fwd(_p(logits), dt, ld, _p(labels), _p(logp), _p(lse), rows, V, ignore_index, inv, _stream()), "ie_logprob_fwd")
+    lse = torch.empty_like(logp)
+    check(_L().ie_logprob_fwd(_ptr(logits), dt, ld, _ptr(labels), _ptr(logp), _ptr(lse), rows, V, ignore_index, inv, stream), "ie_logprob_fwd")
     return logp, lse
+
+
+def _logprob_bwd(logits, labels, on_device, lse, coef, dloss, dloss_mul, ignore_index, temperature, dlogits):
+    """lse, coef: addresses of [rows] fp32; on_device: the tensors they lie in"""
+    rows, V, ld = _logit_rows(logits)
+    _row_vector(labels, rows, torch.int64, "labels")
+    if dloss is not None:
+        _scalar(dloss, "dloss")
+    inv = _inv_temperature(temperature)
+    dlogits, ldd = _dlogits_for(logits, dlogits)
+    dt = _dt(logits)
+    stream = _raw_stream(_on_current_device(logits, labels, dloss, dlogits, *on_device))
+    check(_L().ie_logprob_bwd(_ptr(logits), dt, ld, _ptr(dlogits), ldd, _ptr(labels), lse, coef, _ptr(dloss), dloss_mul, rows, V, ignore_index, inv, stream),
+          "ie_logprob_bwd")
+    return dlogits
 
 
 def token_logprobs_bwd(logits, labels, lse, dlogp, dloss=None, dloss_mul=1.0, ignore_index=-100, temperature=1.0, dlogits=None):
     """Gradient in the logits (in place over them when dlogits is None) of a loss with d loss / d logp = dlogp fp32 [rows]; lse as token_logprobs gave it for
     the same logits, labels and temperature.  dloss (optional, a device scalar: the loss scale) and dloss_mul are factors.  Masked rows are written as zeros."""
-    rows, V, ld = _logit_rows(logits)
-    _row_vector(labels, rows, torch.int64, "labels")
+    rows = logits.shape[0]
     _row_vector(lse, rows, torch.float32, "lse")
     _row_vector(dlogp, rows, torch.float32, "dlogp")
-    if dloss is not None:
-        _scalar(dloss, "dloss")
-    inv = _inv_temperature(temperature)
-    dlogits, ldd = _dlogits_for(logits, dlogits, rows, V)
-    dt = _dt(logits)
-    _on_current_device(logits, labels, lse, dlogp, dloss, dlogits)
-    check(_L().ie_logprob_bwd(_p(logits), dt, ld, _p(dlogits), ldd, _p(labels), _p(lse), _p(dlogp), _p(dloss), dloss_mul, rows, V, ignore_index, inv, _stream()),
-          "ie_logprob_bwd")
-    return dlogits
+    return _logprob_bwd(logits, labels, (lse, dlogp), _ptr(lse), _ptr(dlogp), dloss, dloss_mul, ignore_index, temperature, dlogits)
+
+
+def _loss_bwd(logits, labels, fwd, dloss, dloss_mul, ignore_index, temperature, dlogits):
+    per_row = fwd._rows
+    rows = per_row.shape[1]
+    if logits.shape[0] != rows:
+        raise ValueError(f"the forward call had {rows} rows, logits have {logits.shape[0]}")
+    p = _ptr(per_row)
+    return _logprob_bwd(logits, labels, (per_row,), p + 4 * rows, p + 8 * rows, dloss, dloss_mul, ignore_index, temperature, dlogits)
 
 
 def preference_loss_fwd(logits, labels, cu_seqlens, ref_logps=None, beta=0.1, kind="sigmoid", label_smoothing=0.0, margin=0.0, average=False, ignore_index=-100,
@@ -381,7 +436,7 @@ def preference_loss_fwd(logits, labels, cu_seqlens, ref_logps=None, beta=0.1, ki
     """Paired log-ratio loss over packed answers: cu_seqlens int32 [2 P + 1] on the device, answer 2p chosen over answer 2p + 1.  ref_logps fp32 [2 P]: the
     reference model's summed (average: mean) log-probabilities, None = no reference.  kind "sigmoid" (label_smoothing: probability that a pair is the wrong
     way round), "hinge" or "ipo" (formulas: include/internevo_hip.h).
-    Returns PreferenceLoss(loss [1], rewards [P, 2], seq_logps [2 P], logp, lse, coef [rows]), all fp32; hand it to preference_loss_bwd."""
+    Returns a PreferenceLoss; hand it to preference_loss_bwd."""
     rows, V, ld = _logit_rows(logits)
     _row_vector(labels, rows, torch.int64, "labels")
     seqs = cu_seqlens.numel() - 1
@@ -394,23 +449,23 @@ def preference_loss_fwd(logits, labels, cu_seqlens, ref_logps=None, beta=0.1, ki
         raise ValueError(f"kind: one of {sorted(_PREFERENCE_KINDS)}, not {kind!r}")
     inv = _inv_temperature(temperature)
     dt = _dt(logits)
-    _on_current_device(logits, labels, cu_seqlens, ref_logps)
-    L, dev = _L(), logits.device
-    per_row = torch.empty((3, rows), dtype=torch.float32, device=dev)
-    per_seq = torch.empty((2, seqs), dtype=torch.float32, device=dev)
-    loss = torch.empty(1, dtype=torch.float32, device=dev)
-    ws = torch.empty(L.ie_preference_loss_workspace(seqs // 2), dtype=torch.uint8, device=dev)
-    logp, lse, coef = per_row.unbind(0)
-    rewards, seq_logps = per_seq.unbind(0)
-    check(L.ie_preference_loss_fwd(_p(logits), dt, ld, _p(labels), _p(cu_seqlens), _p(ref_logps), _PREFERENCE_KINDS[kind], beta, label_smoothing, margin,
-                                   int(bool(average)), _p(loss), _p(rewards), _p(seq_logps), _p(logp), _p(lse), _p(coef), _p(ws), rows, V, seqs // 2, ignore_index,
-                                   inv, _stream()), "ie_preference_loss_fwd")
-    return PreferenceLoss(loss, rewards.view(-1, 2), seq_logps, logp, lse, coef)
+    stream = _raw_stream(_on_current_device(logits, labels, cu_seqlens, ref_logps))
+    L = _L()
+    per_row = torch.empty((3, rows), dtype=torch.float32, device=logits.device)
+    ws = L.ie_preference_loss_workspace(seqs // 2) // 4
+    small = per_row.new_empty(2 * seqs + 2 + ws)   # rewards, seq_logps, loss, then (8-byte values: 2 seqs + 2 is even) the workspace
+    p, q = _ptr(per_row), small.data_ptr()
+    step = 4 * rows
+    check(L.ie_preference_loss_fwd(_ptr(logits), dt, ld, _ptr(labels), cu_seqlens.data_ptr(), _ptr(ref_logps), _PREFERENCE_KINDS[kind], beta, label_smoothing, margin,
+                                   bool(average), q + 8 * seqs, q, q + 4 * seqs, p, p + step, p + 2 * step, q + 8 * seqs + 8, rows, V, seqs // 2, ignore_index, inv,
+                                   stream), "ie_preference_loss_fwd")
+    return PreferenceLoss(per_row, small, seqs)
 
 
 def preference_loss_bwd(logits, labels, fwd, dloss=None, dloss_mul=1.0, ignore_index=-100, temperature=1.0, dlogits=None):
-    """Gradient of preference_loss_fwd's loss in the logits (in place over them when dlogits is None); fwd: what the forward call returned."""
-    return token_logprobs_bwd(logits, labels, fwd.lse, fwd.coef, dloss, dloss_mul, ignore_index, temperature, dlogits)
+    """Gradient of preference_loss_fwd's loss in the logits (in place over them when dlogits is None); fwd: what the forward call returned for the same logits, labels,
+    ignore_index and temperature."""
+    return _loss_bwd(logits, labels, fwd, dloss, dloss_mul, ignore_index, temperature, dlogits)
 
 
 def _policy_loss(logits, labels, old_logps, advantages, dloss, dloss_mul, dlogits, ref_logps, clip_low, clip_high, kl_coef, cu_seqlens, ignore_index, temperature):
@@ -432,29 +487,31 @@ def _policy_loss(logits, labels, old_logps, advantages, dloss, dloss_mul, dlogit
     ldd = 0
     if dloss is not None:
         _scalar(dloss, "dloss")
-        dlogits, ldd = _dlogits_for(logits, dlogits, rows, V)
+        dlogits, ldd = _dlogits_for(logits, dlogits)
     dt = _dt(logits)
-    _on_current_device(logits, labels, old_logps, advantages, ref_logps, cu_seqlens, dloss, dlogits)
-    L, dev = _L(), logits.device
-    per_row = torch.empty((3, rows), dtype=torch.float32, device=dev)
-    stats = torch.empty(4, dtype=torch.float32, device=dev)
-    ws = torch.empty(L.ie_policy_loss_workspace(rows, seqs), dtype=torch.uint8, device=dev)
-    logp, lse, coef = per_row.unbind(0)
-    check(L.ie_policy_loss(_p(logits), dt, ld, _p(dlogits), ldd, _p(labels), _p(old_logps), _p(advantages), _p(ref_logps), _p(cu_seqlens), seqs, clip_low, clip_high,
-                           kl_coef, _p(dloss), dloss_mul, _p(stats), _p(logp), _p(lse), _p(coef), _p(ws), rows, V, ignore_index, inv, _stream()), "ie_policy_loss")
-    return PolicyLoss(stats[:1], stats, logp, lse, coef), dlogits
+    stream = _raw_stream(_on_current_device(logits, labels, old_logps, advantages, ref_logps, cu_seqlens, dloss, dlogits))
+    L = _L()
+    per_row = torch.empty((3, rows), dtype=torch.float32, device=logits.device)
+    stats, ws = per_row.new_empty(4), per_row.new_empty(L.ie_policy_loss_workspace(rows, seqs) // 4)
+    p = _ptr(per_row)
+    step = 4 * rows
+    check(L.ie_policy_loss(_ptr(logits), dt, ld, _ptr(dlogits), ldd, _ptr(labels), _ptr(old_logps), _ptr(advantages), _ptr(ref_logps), _ptr(cu_seqlens), seqs, clip_low,
+                           clip_high, kl_coef, _ptr(dloss), dloss_mul, stats.data_ptr(), p, p + step, p + 2 * step, ws.data_ptr(), rows, V, ignore_index, inv,
+                           stream), "ie_policy_loss")
+    return PolicyLoss(per_row, stats), dlogits
 
 
 def policy_loss_fwd(logits, labels, old_logps, advantages, ref_logps=None, clip_low=0.2, clip_high=0.2, kl_coef=0.0, cu_seqlens=None, ignore_index=-100, temperature=1.0):
     """Clipped policy loss with a KL term: -min(r A, clamp(r, 1 - clip_low, 1 + clip_high) A) + kl_coef (e^q - q - 1), r = exp(logp - old_logps), q = ref_logps - logp;
     old_logps, advantages, ref_logps fp32 [rows].  Mean over the rows with a label, or -- cu_seqlens int32 [S + 1] on the device -- the mean over the sequences of
-    each one's mean.  Returns PolicyLoss(loss [1], stats [4] = loss, policy term, KL, clipped share, logp, lse, coef [rows]), all fp32."""
+    each one's mean.  Returns a PolicyLoss; hand it to policy_loss_bwd."""
     return _policy_loss(logits, labels, old_logps, advantages, None, 1.0, None, ref_logps, clip_low, clip_high, kl_coef, cu_seqlens, ignore_index, temperature)[0]
 
 
 def policy_loss_bwd(logits, labels, fwd, dloss=None, dloss_mul=1.0, ignore_index=-100, temperature=1.0, dlogits=None):
-    """Gradient of policy_loss_fwd's loss in the logits (in place over them when dlogits is None); fwd: what the forward call returned."""
-    return token_logprobs_bwd(logits, labels, fwd.lse, fwd.coef, dloss, dloss_mul, ignore_index, temperature, dlogits)
+    """Gradient of policy_loss_fwd's loss in the logits (in place over them when dlogits is None); fwd: what the forward call returned for the same logits, labels,
+    ignore_index and temperature."""
+    return _loss_bwd(logits, labels, fwd, dloss, dloss_mul, ignore_index, temperature, dlogits)
 
 
 def policy_loss_fwd_bwd(logits, labels, old_logps, advantages, dloss, dloss_mul=1.0, dlogits=None, ref_logps=None, clip_low=0.2, clip_high=0.2, kl_coef=0.0,
@@ -467,34 +524,44 @@ def policy_loss_fwd_bwd(logits, labels, old_logps, advantages, dloss, dloss_mul=
 
 
 # ------------------------------------------------------------------------------------------ norm and clipping of a list of gradients
+_dtype_of = operator.attrgetter("dtype")
+
+
 def _tensor_list(tensors, what):
-    """Host arrays (addresses, lengths, types) of a list of contiguous bf16 / fp32 tensors."""
-    for t in tensors:
-        if not t.is_contiguous():
-            raise ValueError(f"{what}: every tensor must be contiguous")
-    return (array.array("q", [t.data_ptr() for t in tensors]), array.array("q", [t.numel() for t in tensors]), array.array("i", [_dt(t) for t in tensors]))
+    """Host arrays (addresses, lengths, types) of a list of contiguous bf16 / fp32 tensors on the current device.  map() over the methods themselves: a list of
+    hundreds is most of such a call's time."""
+    T = torch.Tensor
+    if not tensors:
+        raise ValueError(f"{what}: an empty list")
+    if not all(map(T.is_contiguous, tensors)):
+        raise ValueError(f"{what}: every tensor must be contiguous")
+    try:
+        dtypes = array.array("i", list(map(_DT.__getitem__, map(_dtype_of, tensors))))
+    except KeyError as e:
+        raise ValueError(f"{what}: unsupported dtype {e.args[0]}") from None
+    return array.array("q", list(map(T.data_ptr, tensors))), array.array("q", list(map(T.numel, tensors))), dtypes
+
+
+def _list_device(tensors, what):
+    index = set(map(torch.Tensor.get_device, tensors))
+    if len(index) > 1:
+        raise ValueError(f"{what}: tensors on different devices")
+    return _on_current_device(tensors[0])
 
 
 def _addr(a):
-    return ctypes.c_void_p(a.buffer_info()[0])
+    return a.buffer_info()[0]
 
 
 def grad_norm(tensors):
     """L2 norm over a list of bf16 / fp32 tensors of any lengths -> fp32[1] on the device; squares and sums in 64 bits, fixed order."""
     tensors = list(tensors)
-    if not tensors:
-        raise ValueError("grad_norm: an empty list")
-    return _grad_norm(tensors, _tensor_list(tensors, "grad_norm"))
-
-
-def _grad_norm(tensors, lists):
-    _on_current_device(*tensors)
-    _p(tensors[0])   # (refuses host tensors)
-    L, dev, n = _L(), tensors[0].device, len(tensors)
-    ws = torch.empty(L.ie_grad_norm_workspace(n), dtype=torch.uint8, device=dev)
-    norm = torch.empty(1, dtype=torch.float32, device=dev)
-    ptrs, numels, dtypes = lists
-    check(L.ie_grad_norm(_addr(ptrs), _addr(numels), _addr(dtypes), n, _p(ws), _p(norm), _stream()), "ie_grad_norm")
+    ptrs, numels, dtypes = _tensor_list(tensors, "grad_norm")
+    stream = _raw_stream(_list_device(tensors, "grad_norm"))
+    L, n = _L(), len(tensors)
+    norm = torch.empty(1, dtype=torch.float32, device=tensors[0].device)
+    ws = norm.new_empty(L.ie_grad_norm_workspace(n) // 4)
+    check(L.ie_grad_norm(_addr(ptrs), _addr(numels), _addr(dtypes), n, ws.data_ptr(), norm.data_ptr(), stream), "ie_grad_norm")
     return norm
 
 
@@ -503,23 +570,23 @@ def clip_grad_norm_(tensors, max_norm, out=None):
     fp32[1] on the device; no host synchronisation.  In place, or into `out`: a list of contiguous tensors of the same lengths, bf16 or fp32 (the optimizer's fp32
     gradients), apart from the inputs.  A tensor named twice, or overlapping another one that is written, is refused."""
     tensors = list(tensors)
-    if not tensors:
-        raise ValueError("clip_grad_norm_: an empty list")
     if not max_norm >= 0:
         raise ValueError(f"clip_grad_norm_: max_norm must not be negative ({max_norm})")
-    lists = _tensor_list(tensors, "clip_grad_norm_")
-    optrs = odtypes = None
+    ptrs, numels, dtypes = _tensor_list(tensors, "clip_grad_norm_")
+    every, optrs, odtypes = tensors, None, None
     if out is not None:
         out = list(out)
-        optrs, onumels, odtypes = _tensor_list(out, "clip_grad_norm_: out")
-        if onumels != lists[1]:
+        if len(out) == len(tensors):
+            optrs, onumels, odtypes = _tensor_list(out, "clip_grad_norm_: out")
+        if optrs is None or onumels != numels:
             raise ValueError("clip_grad_norm_: out must hold one tensor of the same length for every input")
-        _on_current_device(tensors[0], *out)
-    norm = _grad_norm(tensors, lists)
-    ptrs, numels, dtypes = lists
-    none = ctypes.c_void_p(0)
-    check(_L().ie_grad_clip(_addr(ptrs), _addr(numels), _addr(dtypes), _addr(optrs) if out is not None else none, _addr(odtypes) if out is not None else none,
-                            len(tensors), _p(norm), float(max_norm), _stream()), "ie_grad_clip")
+        every = tensors + out
+    stream = _raw_stream(_list_device(every, "clip_grad_norm_"))
+    L, n = _L(), len(tensors)
+    norm = torch.empty(1, dtype=torch.float32, device=tensors[0].device)
+    ws = norm.new_empty(L.ie_grad_norm_workspace(n) // 4)
+    check(L.ie_grad_clip(_addr(ptrs), _addr(numels), _addr(dtypes), _addr(optrs) if out is not None else None, _addr(odtypes) if out is not None else None, n,
+                         float(max_norm), ws.data_ptr(), norm.data_ptr(), stream), "ie_grad_clip")
     return norm
 
 

@@ -202,7 +202,7 @@ def test_gradient_list_entries_refuse_bad_calls(lib):
         n = len(ptrs)
         o = (ctypes.c_void_p * n)(*outs) if outs else None
         d = (ctypes.c_int * n)(*odt) if odt else None
-        return lib.ie_grad_clip(*_arrays(ptrs, numels, dtypes), o, d, n, norm, max_norm, None)
+        return lib.ie_grad_clip(*_arrays(ptrs, numels, dtypes), o, d, n, max_norm, FAKE, norm, None)
 
     _refused(lib, clip([4096], [8], [0], norm=None), "null")
     _refused(lib, clip([4096], [8], [0], max_norm=-1.0), "max_norm")
@@ -218,6 +218,6 @@ def test_gradient_list_entries_refuse_bad_calls(lib):
 
 def test_workspace_sizes(lib):
     assert lib.ie_preference_loss_workspace(3) == 24
-    assert lib.ie_policy_loss_workspace(10, 0) == 31 * 4 and lib.ie_policy_loss_workspace(10, 4) == 34 * 4
+    assert lib.ie_policy_loss_workspace(10, 0) == 41 * 4 and lib.ie_policy_loss_workspace(10, 4) == 44 * 4
     # one launch at least, and one more for every full set of tensors
     assert lib.ie_grad_norm_workspace(0) > 0 and lib.ie_grad_norm_workspace(1000) > lib.ie_grad_norm_workspace(1)
