@@ -89,10 +89,12 @@ def draw(rng):
         if not odd:
             hidden = hidden // 8 * 8
         ffn, kv = int(hidden * rng.uniform(2.0, 3.5)), max(1, hidden // rng.choice([1, 2, 4, 8]))
-        layers = _spread(rng, 1, max(1, min(60, int(4.5e8 / (hidden * (2 * hidden + 2 * kv + 3 * ffn))))))
+        form = rng.choice(["clip", "clip", "norm"])
+        most = 60 if form == "norm" else 8   # every clipped tensor is an output: 59 at most
+        layers = _spread(rng, 1, max(1, min(most, int(4.5e8 / (hidden * (2 * hidden + 2 * kv + 3 * ffn))))))
         vocab = rng.choice([0, _spread(rng, 100, max(101, min(92544, int(7e7 / hidden))))])
         return _clip(None, hidden, layers, ffn, vocab, kv, grads=rng.choice(["bf16", "fp32", "mixed"]),
-                     out=rng.choice(["bf16", "fp32"]), form=rng.choice(["clip", "clip", "norm"]), odd=odd, max_norm=rng.choice([0.5, 1.0, 1e6]))
+                     out=rng.choice(["bf16", "fp32"]), form=form, odd=odd, max_norm=rng.choice([0.5, 1.0, 1e6]))
     vocab = rng.choice([32000, 92544, 103168, _spread(rng, 500, 131072), _spread(rng, 500, 131072)])
     dtype = rng.choice(["bf16", "bf16", "fp32"])
     tokens = _spread(rng, 1 if op != "preference" else 4, max(8, min(16384, int((7e8 if dtype == "bf16" else 3.5e8) / vocab))))
