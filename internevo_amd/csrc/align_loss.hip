@@ -65,59 +65,81 @@ template <bool S> __device__ __forceinline__ void stv(void* p, const u32x4& v) {
     else *(u32x4_any*)p = v;
 }
 
-// Maximum m of a row and s = sum 2^((x - m) k), k = log2(e) / tau, in one pass: 2^((m_old - m_new) k) rescales what was summed before a new maximum.  The difference
-// is taken before the product: it is exact next to the maximum, and logits masked by the type's lowest value cannot overflow into inf - inf.  While nothing but
-// -inf has been seen the reference is 0, so that such logits add 0; NaN and +inf make s NaN.
-__device__ __forceinline__ float max_ref(float m) { return m == -INFINITY ? 0.f : m; }
-__device__ __forceinline__ float rescale(float m_old, float m_new, float k) { return m_old == -INFINITY ? 0.f : exp2_((m_old - max_ref(m_new)) * k); }
+// Sums of exponentials.  With k = log2(e) / tau:  exp((x - m) / tau) = 2^(x k - r), r = fl(m k): one fma and one exponential an element, m the largest logit so far; what
+// rounding m k loses is the same factor in every term and is taken out of the logarithm at the end (it cancels in p).  The form fails where x k leaves fp32 -- rows in
+// which no logit is above -1e30, such as a vocabulary masked as a whole by the type's lowest value, or whose largest is +inf: those are done over as 2^((x - m) k) (F = false).
+// A maximum that cannot serve counts as none: reference 0, and every term it would belong to is 0 beside any other logit.  NaN and +inf make the sum NaN.
+constexpr float kRange = 1e30f;
+__device__ __forceinline__ float ref(float m, float k) { return m * k >= -kRange ? m * k : 0.f; }
+__device__ __forceinline__ bool in_range(float m, float k) { return fabsf(m * k) <= kRange; }
+template <bool F> __device__ __forceinline__ float term(float x, float k, float r) { return exp2_(F ? __builtin_fmaf(x, k, -r) : (x - r) * k); }
+// sum s of terms that belong to reference r, brought to reference to >= r
+__device__ __forceinline__ float bring(float s, float r, float to) { return s == 0.f ? 0.f : s * exp2_(r - to); }
 
 struct RowStat {
-    float m, s;
+    float m, r, s;   // r: reference of s, m k (fast) or m itself
+    bool fast;
     // log sum exp((x - m) / tau): the exponent of s apart, so that only the logarithm of a number next to 1 is rounded to 32 bits
-    __device__ __forceinline__ double log_sum() const {
+    __device__ __forceinline__ double log_sum(float k) const {
         int e;
         float f = frexpf(s, &e);
         if (!(f > 0.f) || f == INFINITY) return (double)logf(s);
         if (f < 0.70710678f) { f *= 2.f; --e; }
-        return (double)e * kLn2 + (double)logf(f);
+        return (double)e * kLn2 + (double)logf(f) - (fast ? ((double)m * (double)k - (double)r) * kLn2 : 0.0);
     }
-    __device__ __forceinline__ double lse(double inv_tau) const { return (double)m * inv_tau + log_sum(); }
-    __device__ __forceinline__ double logp(float x, double inv_tau) const { return ((double)x - (double)m) * inv_tau - log_sum(); }
+    __device__ __forceinline__ double lse(double inv_tau, float k) const { return (double)m * inv_tau + log_sum(k); }
+    __device__ __forceinline__ double logp(float x, double inv_tau, float k) const { return ((double)x - (double)m) * inv_tau - log_sum(k); }
 };
 
-// (m, s) of every thread -> of the workgroup; every thread returns the same.  sh: 2 NT / 64 floats.
+// (m, s) of every thread, s at reference ref(m), -> of the workgroup; every thread returns the same.  sh: 2 NT / 64 floats.
 template <int NT>
 __device__ __forceinline__ RowStat join_stats(float m, float s, float k, float* sh) {
     constexpr int NW = NT / 64;
     const float wm = wave_max(m);
-    s = wave_sum(s * rescale(m, wm, k));
-    if (NW == 1) return {wm, s};
+    s = wave_sum(bring(s, ref(m, k), ref(wm, k)));
+    if (NW == 1) return {wm, ref(wm, k), s, in_range(wm, k)};
     if ((threadIdx.x & 63) == 0) { sh[threadIdx.x >> 6] = wm; sh[NW + (threadIdx.x >> 6)] = s; }
     __syncthreads();
     m = sh[threadIdx.x & (NW - 1)];
     float b = m;
 #pragma unroll
     for (int o = NW / 2; o > 0; o >>= 1) b = fmaxf(b, __shfl_xor(b, o, 64));
-    s = sh[NW + (threadIdx.x & (NW - 1))] * rescale(m, b, k);
+    s = bring(sh[NW + (threadIdx.x & (NW - 1))], ref(m, k), ref(b, k));
 #pragma unroll
     for (int o = NW / 2; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
-    return {b, s};
+    return {b, ref(b, k), s, in_range(b, k)};
 }
 
-template <bool BF>
-__device__ __forceinline__ void add_values(const float* v, int n, float k, float& m, float& s) {
+template <int N>
+__device__ __forceinline__ void add_values(const float* v, float k, float& m, float& s) {
     float c = v[0];
 #pragma unroll
-    for (int e = 1; e < n; ++e) c = fmaxf(c, v[e]);
-    if (c > m) { s *= rescale(m, c, k); m = c; }
-    const float r = max_ref(m);
+    for (int e = 1; e < N; ++e) c = fmaxf(c, v[e]);
+    if (c > m) { s = bring(s, ref(m, k), ref(c, k)); m = c; }
+    const float r = ref(m, k);
 #pragma unroll
-    for (int e = 0; e < n; ++e) s += exp2_((v[e] - r) * k);
+    for (int e = 0; e < N; ++e) s += term<true>(v[e], k, r);
+}
+
+// The row whose maximum m is out of the fast form's range, again.  sh as in join_stats, free to be written after the barrier at its start.
+template <bool BF, int NT>
+__device__ __noinline__ RowStat row_stat_again(const typename Elem<BF>::T* x, int vocab, float m, float k, float* sh) {
+    constexpr int NW = NT / 64;
+    const float r = m == -INFINITY ? 0.f : m;
+    float s = 0.f;
+    for (int i = threadIdx.x; i < vocab; i += NT) s += term<false>(Elem<BF>::get(x + i), k, r);
+    s = wave_sum(s);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = s;
+    __syncthreads();
+    s = 0.f;
+    for (int w = 0; w < NW; ++w) s += sh[w];
+    return {m, r, s, false};
 }
 
 // One pass over the row, U 16-byte loads a thread in flight.
 template <bool BF, int NT, int U, bool S>
-__device__ __forceinline__ RowStat row_stat(const typename Elem<BF>::T* __restrict__ x, int vocab, float k, float* sh) {
+__device__ __forceinline__ RowStat row_stat(const typename Elem<BF>::T* x, int vocab, float k, float* sh) {
     constexpr int N = Elem<BF>::N;
     float m = -INFINITY, s = 0.f;
     const int nv = vocab / N;
@@ -129,9 +151,9 @@ __device__ __forceinline__ RowStat row_stat(const typename Elem<BF>::T* __restri
         float v[U * N];
 #pragma unroll
         for (int u = 0; u < U; ++u) Elem<BF>::unpack(w[u], v + u * N);
-        add_values<BF>(v, U * N, k, m, s);
+        add_values<U * N>(v, k, m, s);
     }
-    if (U > 1 && i < nv) {   // fewer than U vectors left: loaded together too, what is not there stays -inf
+    if (i < nv) {   // fewer than U vectors left: loaded together too, what is not there stays -inf
         u32x4 w[U - 1];
 #pragma unroll
         for (int u = 0; u < U - 1; ++u) {
@@ -142,14 +164,15 @@ __device__ __forceinline__ RowStat row_stat(const typename Elem<BF>::T* __restri
         for (int u = 0; u < U - 1; ++u) {
             float v[N];
             Elem<BF>::unpack(w[u], v);
-            add_values<BF>(v, N, k, m, s);
+            add_values<N>(v, k, m, s);
         }
     }
     if ((int)threadIdx.x < vocab - nv * N) {
         const float v = Elem<BF>::get(x + nv * N + threadIdx.x);
-        add_values<BF>(&v, 1, k, m, s);
+        add_values<1>(&v, k, m, s);
     }
-    return join_stats<NT>(m, s, k, sh);
+    const RowStat st = join_stats<NT>(m, s, k, sh);
+    return st.fast ? st : row_stat_again<BF, NT>(x, vocab, st.m, k, sh);
 }
 
 __device__ __forceinline__ bool row_label(const int64_t* labels, int64_t row, int64_t ignore_index, int vocab, int& lab) {
@@ -166,19 +189,19 @@ __device__ __forceinline__ bool owns(int lab, int vocab) {
     return (int)threadIdx.x == (lab < nv * N ? (lab / N) % NT : lab - nv * N);
 }
 
-template <bool BF>
-__device__ __forceinline__ u32x4 grad_vector(const u32x4& w, float k, float m, float g_p) {
+template <bool BF, bool F>
+__device__ __forceinline__ u32x4 grad_vector(const u32x4& w, float k, float r, float g_p) {
     float v[Elem<BF>::N];
     Elem<BF>::unpack(w, v);
 #pragma unroll
-    for (int e = 0; e < Elem<BF>::N; ++e) v[e] = -g_p * exp2_((v[e] - m) * k);
+    for (int e = 0; e < Elem<BF>::N; ++e) v[e] = -g_p * term<F>(v[e], k, r);
     return Elem<BF>::pack(v);
 }
 
-// d = g 1[j = label] - g_p 2^((x - m) k) for the whole row: with the row's maximum and sum g_p = g / s, with its log-sum-exp in m's place g_p = g.  xl: the label's
+// d = g 1[j = label] - g_p 2^(x k - r) for the whole row: with the row's reference and sum g_p = g / s, with its log-sum-exp as reference g_p = g.  xl: the label's
 // logit, read before any store (dlogits may be the logits themselves).
-template <bool BF, int NT, int U, bool S>
-__device__ __forceinline__ void row_grad(const typename Elem<BF>::T* x, typename Elem<BF>::T* d, int vocab, float k, float m, float g, float g_p, int lab, float xl) {
+template <bool BF, int NT, int U, bool S, bool F>
+__device__ __forceinline__ void row_grad(const typename Elem<BF>::T* x, typename Elem<BF>::T* d, int vocab, float k, float r, float g, float g_p, int lab, float xl) {
     constexpr int N = Elem<BF>::N;
     const int nv = vocab / N;
     int i = threadIdx.x;
@@ -187,18 +210,26 @@ __device__ __forceinline__ void row_grad(const typename Elem<BF>::T* x, typename
 #pragma unroll
         for (int u = 0; u < U; ++u) w[u] = ldv<S>(x + (int64_t)(i + u * NT) * N);
 #pragma unroll
-        for (int u = 0; u < U; ++u) stv<S>(d + (int64_t)(i + u * NT) * N, grad_vector<BF>(w[u], k, m, g_p));
+        for (int u = 0; u < U; ++u) stv<S>(d + (int64_t)(i + u * NT) * N, grad_vector<BF, F>(w[u], k, r, g_p));
     }
-    u32x4 w[U - 1];
+    if (U > 1) {
+        u32x4 w[U];
 #pragma unroll
-    for (int u = 0; u < U - 1; ++u)
-        if (i + u * NT < nv) w[u] = ldv<S>(x + (int64_t)(i + u * NT) * N);
+        for (int u = 0; u < U - 1; ++u)
+            if (i + u * NT < nv) w[u] = ldv<S>(x + (int64_t)(i + u * NT) * N);
 #pragma unroll
-    for (int u = 0; u < U - 1; ++u)
-        if (i + u * NT < nv) stv<S>(d + (int64_t)(i + u * NT) * N, grad_vector<BF>(w[u], k, m, g_p));
+        for (int u = 0; u < U - 1; ++u)
+            if (i + u * NT < nv) stv<S>(d + (int64_t)(i + u * NT) * N, grad_vector<BF, F>(w[u], k, r, g_p));
+    }
     i = nv * N + threadIdx.x;
-    if (i < vocab) Elem<BF>::put(d + i, -g_p * exp2_((Elem<BF>::get(x + i) - m) * k));
-    if (owns<BF, NT>(lab, vocab)) Elem<BF>::put(d + lab, g - g_p * exp2_((xl - m) * k));
+    if (i < vocab) Elem<BF>::put(d + i, -g_p * term<F>(Elem<BF>::get(x + i), k, r));
+    if (owns<BF, NT>(lab, vocab)) Elem<BF>::put(d + lab, g - g_p * term<F>(xl, k, r));
+}
+
+// the same for a row out of the fast form's range
+template <bool BF, int NT>
+__device__ __noinline__ void row_grad_again(const typename Elem<BF>::T* x, typename Elem<BF>::T* d, int vocab, float k, float r, float g, float g_p, int lab, float xl) {
+    row_grad<BF, NT, 1, false, false>(x, d, vocab, k, r, g, g_p, lab, xl);
 }
 
 template <bool BF, int NT, bool S>
@@ -224,10 +255,11 @@ __global__ __launch_bounds__(NT) void logprob_fwd_k(const void* __restrict__ log
     }
     const typename Elem<BF>::T* x = (const typename Elem<BF>::T*)logits + row * ld;
     const float xl = Elem<BF>::get(x + lab);
-    const RowStat st = row_stat<BF, NT, 4, S>(x, vocab, (float)(inv_tau * kLog2e), sh);
+    const float k = (float)(inv_tau * kLog2e);
+    const RowStat st = row_stat<BF, NT, 4, S>(x, vocab, k, sh);
     if (threadIdx.x == 0) {
-        lse[row] = (float)st.lse(inv_tau);
-        logp[row] = (float)st.logp(xl, inv_tau);
+        lse[row] = (float)st.lse(inv_tau, k);
+        logp[row] = (float)st.logp(xl, inv_tau, k);
         if (coef) coef[row] = 0.f;
     }
 }
@@ -247,18 +279,18 @@ __global__ __launch_bounds__(NT) void logprob_bwd_k(const void* logits, int64_t 
     const float k = (float)(inv_tau * kLog2e);
     const typename Elem<BF>::T* x = (const typename Elem<BF>::T*)logits + row * ld;
     const float xl = Elem<BF>::get(x + lab);
-    // p = 2^((x - l) k), l = lse tau: what rounding l to 32 bits loses goes into the factor
-    const double l = (double)lse[row] / inv_tau;
-    float m = (float)l, g_p = g;
-    if (m < -1e30f) {   // every logit at the type's lowest value or below: there the log-sum-exp cannot hold the sum beside the maximum
+    // p = 2^(x k - l k), l = lse tau: what rounding l k to 32 bits loses goes into the factor
+    const double l = (double)lse[row] / inv_tau * (double)k;
+    const float r = (float)l;
+    if (fabsf(r) <= kRange) {
+        const float g_p = g * exp2_((float)((double)r - l));
+        __syncthreads();   // xl is read before another wave's stores may replace it
+        row_grad<BF, NT, U, S, true>(x, d, vocab, k, r, g, g_p, lab, xl);
+    } else {   // out of the fast form's range, where the log-sum-exp cannot hold the sum beside the maximum
         const RowStat st = row_stat<BF, NT, 4, S>(x, vocab, k, sh);
-        m = st.m;
-        g_p = g / st.s;
-    } else {
-        g_p *= exp2_((float)((double)m - l) * k);
+        __syncthreads();
+        row_grad_again<BF, NT>(x, d, vocab, k, st.r, g, g / st.s, lab, xl);
     }
-    __syncthreads();   // xl is read before another wave's stores may replace it
-    row_grad<BF, NT, U, S>(x, d, vocab, k, m, g, g_p, lab, xl);
 }
 
 // ------------------------------------------------------------------------------------------ sums over a workgroup in 64 bits, fixed order
@@ -443,18 +475,22 @@ __device__ __forceinline__ float policy_weight(const PolicyArgs& a, bool inside,
     return inside ? (float)(1.0 / ((a.cu ? (double)a.seqs : 1.0) * (double)max(n, 1))) : 0.f;
 }
 
+struct PolicyRow {
+    float old, adv, ref;
+};
+__device__ __forceinline__ PolicyRow policy_row(const PolicyArgs& a, int64_t t) { return {a.old_logps[t], a.adv[t], a.ref ? a.ref[t] : 0.f}; }
+
 // terms of one row and d loss / d logp; the log-ratios are differences of 64-bit values, so that they alone are rounded
-__device__ __forceinline__ float policy_term(const PolicyArgs& a, int64_t t, double logp, float w, float4& term) {
+__device__ __forceinline__ float policy_term(const PolicyArgs& a, const PolicyRow& in, double logp, float w, float4& term) {
     term = make_float4(0.f, 0.f, 0.f, 0.f);
     if (w == 0.f) return 0.f;
-    const float adv = a.adv[t];
-    const float ratio = expf((float)(logp - (double)a.old_logps[t]));
-    const bool clipped = (adv > 0.f && ratio > 1.f + a.high) || (adv < 0.f && ratio < 1.f - a.low);
-    const float bound = adv > 0.f ? 1.f + a.high : 1.f - a.low;
-    const float s = -(clipped ? bound : ratio) * adv;
-    float d = clipped ? 0.f : -ratio * adv, kl = 0.f;
+    const float ratio = expf((float)(logp - (double)in.old));
+    const bool clipped = (in.adv > 0.f && ratio > 1.f + a.high) || (in.adv < 0.f && ratio < 1.f - a.low);
+    const float bound = in.adv > 0.f ? 1.f + a.high : 1.f - a.low;
+    const float s = -(clipped ? bound : ratio) * in.adv;
+    float d = clipped ? 0.f : -ratio * in.adv, kl = 0.f;
     if (a.ref) {
-        const float q = (float)((double)a.ref[t] - logp), e = expm1f(q);
+        const float q = (float)((double)in.ref - logp), e = expm1f(q);
         kl = e - q;
         if (a.kl_coef > 0.f) d -= a.kl_coef * e;   // (0 * inf would turn a mere report into NaN)
     }
@@ -470,7 +506,7 @@ __global__ __launch_bounds__(256) void policy_terms_k(PolicyArgs a, const float*
     const bool valid = row_label(a.labels, t, a.ignore_index, a.vocab, lab);
     int64_t s = 0, begin, end;
     const bool inside = valid && policy_range(a, t, s, begin, end);
-    if ((threadIdx.x & 63) == 0) a.coef[t] = policy_term(a, t, (double)logp[t], policy_weight(a, inside, inside ? a.counts[s] : 0), a.terms[t]);
+    if ((threadIdx.x & 63) == 0) a.coef[t] = policy_term(a, policy_row(a, t), (double)logp[t], policy_weight(a, inside, inside ? a.counts[s] : 0), a.terms[t]);
 }
 
 __device__ __forceinline__ void write_stats(const double* v, float kl_coef, float* stats) {
@@ -517,16 +553,17 @@ __global__ __launch_bounds__(1024) void policy_small_k(PolicyArgs a, const float
         const int64_t t = (int64_t)q * 1024 + threadIdx.x;
         if (t >= a.rows) continue;
         float4 term = make_float4(0.f, 0.f, 0.f, 0.f);
-        a.coef[t] = seq[q] < 0 ? 0.f : policy_term(a, t, (double)logp[t], policy_weight(a, true, a.cu ? cnt[seq[q]] : n), term);
+        a.coef[t] = seq[q] < 0 ? 0.f : policy_term(a, policy_row(a, t), (double)logp[t], policy_weight(a, true, a.cu ? cnt[seq[q]] : n), term);
         v[0] += (double)term.x; v[1] += (double)term.y; v[2] += (double)term.z;
     }
     for (int c = 0; c < 3; ++c) v[c] = block_sum_d<16>(v[c], scratch);
     if (threadIdx.x == 0) write_stats(v, a.kl_coef, stats);
 }
 
-// Forward and backward of one row: its coefficient needs nothing but the row itself, so the logits are read once.  NV > 0: the row waits in registers, NV vectors a
-// thread; NV = 0 (longer rows): it is read again, from the last-level cache.
-template <bool BF, int NT, int NV, bool S>
+// Forward and backward of one row: its coefficient needs nothing but the row itself, so the logits are read once.  The row waits in registers, NV
+// vectors a thread (0: longer rows, read again from the last-level cache).  HELD: what waits are its exponentials in 32 bits; otherwise the logits, packed, which are
+// raised a second time.
+template <bool BF, int NT, int NV, bool HELD, bool S>
 __global__ __launch_bounds__(NT) void policy_fused_k(PolicyArgs a, const void* logits, int64_t ld, void* dlogits, int64_t ldd, float* __restrict__ logp_out,
                                                      float* __restrict__ lse_out, const float* __restrict__ dloss, float dloss_mul, double inv_tau) {
     typedef typename Elem<BF>::T T;
@@ -543,28 +580,37 @@ __global__ __launch_bounds__(NT) void policy_fused_k(PolicyArgs a, const void* l
         row_zero<BF, NT, S>(d, vocab);
         return;
     }
-    // no counts (rows <= kCountRows NT): this workgroup's threads look at all labels, before the row's own loads
+    // everything the coefficient will need is asked for before the row's own loads, which it would otherwise wait behind
+    const PolicyRow in = policy_row(a, row);
+    const float scale = dloss_mul * dloss[0] * (float)inv_tau;
+    int64_t seq, begin, end;
+    const bool inside = policy_range(a, row, seq, begin, end);
+    int n = 0;
     unsigned live = 0;
-    if (!a.counts) {
+    if (a.counts) {
+        n = inside ? a.counts[seq] : 0;
+    } else {   // no counts (rows <= kCountRows NT): this workgroup's threads look at all labels
 #pragma unroll
         for (int q = 0; q < kCountRows; ++q) {
             const int64_t t = (int64_t)q * NT + threadIdx.x;
             int other;
-            if (t < a.rows && row_label(a.labels, t, a.ignore_index, vocab, other)) live |= 1u << q;
+            if (t < end && row_label(a.labels, t, a.ignore_index, vocab, other) && t >= begin) live |= 1u << q;
         }
     }
     const T* x = (const T*)logits + row * ld;
     const float xl = Elem<BF>::get(x + lab);
     const float k = (float)(inv_tau * kLog2e);
     const int nv = vocab / N;
-    u32x4 v[NV > 0 ? NV : 1];
+    constexpr int NR = NV > 0 ? NV : 1;
+    u32x4 v[NR];
+    float ex[HELD ? NR * N : 1], ex_rest = 0.f, own = 0.f;   // own: reference of the thread's terms
     RowStat st;
     if (NV > 0) {
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
             const int i = threadIdx.x + j * NT;
             v[j] = Elem<BF>::ninf();
-            if (i < nv) v[j] = ldv<S>(x + (int64_t)i * N);
+            if (i < nv) v[j] = ldv<true>(x + (int64_t)i * N);   // (read once)
         }
         float rest = -INFINITY;
         if (nv * N + (int)threadIdx.x < vocab) rest = Elem<BF>::get(x + nv * N + threadIdx.x);
@@ -574,37 +620,42 @@ __global__ __launch_bounds__(NT) void policy_fused_k(PolicyArgs a, const void* l
             float e[N];
             Elem<BF>::unpack(v[j], e);
 #pragma unroll
-            for (int q = 0; q < N; ++q) m = fmaxf(m, e[q]);
+            for (int q = 0; q < N; ++q) {
+                m = fmaxf(m, e[q]);
+                if (HELD) ex[j * N + q] = e[q];
+            }
         }
         // the vectors stay packed from pass to pass: kept unpacked they would not fit
+        if (!HELD) {
 #pragma unroll
-        for (int j = 0; j < NV; ++j) asm volatile("" : "+v"(v[j]));
-        const float r = max_ref(m);
-        float s = exp2_((rest - r) * k);
+            for (int j = 0; j < NV; ++j) asm volatile("" : "+v"(v[j]));
+        }
+        own = ref(m, k);
+        float s = ex_rest = term<true>(rest, k, own);
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
             float e[N];
-            Elem<BF>::unpack(v[j], e);
+            if (!HELD) Elem<BF>::unpack(v[j], e);
 #pragma unroll
-            for (int q = 0; q < N; ++q) s += exp2_((e[q] - r) * k);
+            for (int q = 0; q < N; ++q) {
+                const float z = term<true>(HELD ? ex[j * N + q] : e[q], k, own);
+                s += z;
+                if (HELD) ex[j * N + q] = z;
+            }
         }
+        if (!HELD) {
 #pragma unroll
-        for (int j = 0; j < NV; ++j) asm volatile("" : "+v"(v[j]));
+            for (int j = 0; j < NV; ++j) asm volatile("" : "+v"(v[j]));
+        }
         st = join_stats<NT>(m, s, k, sh);
+        own = m * k >= -kRange ? exp2_(own - st.r) : 0.f;   // now: the factor of the thread's terms
+        if (!st.fast) st = row_stat_again<BF, NT>(x, vocab, st.m, k, sh);
     } else {
         st = row_stat<BF, NT, 4, false>(x, vocab, k, sh);
     }
-    int64_t seq, begin, end;
-    const bool inside = policy_range(a, row, seq, begin, end);
-    int n = 0;
-    if (a.counts) {
-        n = inside ? a.counts[seq] : 0;
-    } else {
+    if (!a.counts) {
 #pragma unroll
-        for (int q = 0; q < kCountRows; ++q) {
-            const int64_t t = (int64_t)q * NT + threadIdx.x;
-            n += __popcll(__ballot((live >> q & 1u) && t >= begin && t < end));
-        }
+        for (int q = 0; q < kCountRows; ++q) n += __popcll(__ballot(live >> q & 1u));
         if ((threadIdx.x & 63) == 0) counted[threadIdx.x >> 6] = n;
         __syncthreads();
         n = 0;
@@ -612,26 +663,38 @@ __global__ __launch_bounds__(NT) void policy_fused_k(PolicyArgs a, const void* l
         for (int w = 0; w < NT / 64; ++w) n += counted[w];
     }
     if (threadIdx.x == 0) {
-        const double logp = st.logp(xl, inv_tau);
+        const double logp = st.logp(xl, inv_tau, k);
         logp_out[row] = (float)logp;
-        lse_out[row] = (float)st.lse(inv_tau);
-        coef_sh = a.coef[row] = policy_term(a, row, logp, policy_weight(a, inside, n), a.terms[row]);
+        lse_out[row] = (float)st.lse(inv_tau, k);
+        coef_sh = a.coef[row] = policy_term(a, in, logp, policy_weight(a, inside, n), a.terms[row]);
     }
     __syncthreads();
-    const float g = coef_sh * dloss_mul * dloss[0] * (float)inv_tau;
+    const float g = coef_sh * scale;
     if (g == 0.f) { row_zero<BF, NT, S>(d, vocab); return; }
     const float g_p = g / st.s;
-    if (NV > 0) {
+    if (!st.fast) {
+        row_grad_again<BF, NT>(x, d, vocab, k, st.r, g, g_p, lab, xl);
+    } else if (NV > 0) {
+        const float f = -g_p * own;
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
             const int i = threadIdx.x + j * NT;
-            if (i < nv) stv<S>(d + (int64_t)i * N, grad_vector<BF>(v[j], k, st.m, g_p));
+            if (i >= nv) continue;
+            u32x4 out;
+            if (HELD) {
+                float e[N];
+#pragma unroll
+                for (int q = 0; q < N; ++q) e[q] = f * ex[j * N + q];
+                out = Elem<BF>::pack(e);
+            } else {
+                out = grad_vector<BF, true>(v[j], k, st.r, g_p);
+            }
+            stv<S>(d + (int64_t)i * N, out);
         }
-        const int i = nv * N + threadIdx.x;
-        if (i < vocab) Elem<BF>::put(d + i, -g_p * exp2_((Elem<BF>::get(x + i) - st.m) * k));
-        if (owns<BF, NT>(lab, vocab)) Elem<BF>::put(d + lab, g - g_p * exp2_((xl - st.m) * k));
+        if (nv * N + (int)threadIdx.x < vocab) Elem<BF>::put(d + nv * N + threadIdx.x, f * ex_rest);
+        if (owns<BF, NT>(lab, vocab)) Elem<BF>::put(d + lab, g - g_p * term<true>(xl, k, st.r));
     } else {
-        row_grad<BF, NT, 4, S>(x, d, vocab, k, st.m, g, g_p, lab, xl);
+        row_grad<BF, NT, 4, S, true>(x, d, vocab, k, st.r, g, g_p, lab, xl);
     }
 }
 
@@ -675,35 +738,40 @@ struct Launch {
     template <int NT, typename F, typename... A> void go(F f, A... args) const { hipLaunchKernelGGL(f, dim3((unsigned)rows), dim3(NT), 0, st, args...); }
 };
 
+// Threads a row.  Forward, 8000 x 4000 bf16: 64 threads 17.3 us, 256 17.8, 512 31; 2000 x 32 000 bf16: 256 22.0, 512 22.6, 1024 24.0; 3001 x 32 003 fp32: 256 54, 512 49,
+// 1024 48; 16 384 x 92 544 bf16: 256 266, 512 259, 1024 260; with fewer rows than two a CU the widest workgroup is the shortest wait.
 template <bool BF, bool S>
 void launch_fwd(const Launch& l, int nv, const void* logits, int64_t ld, const int64_t* labels, float* logp, float* lse, float* coef, int vocab, int64_t ignore_index, double inv_tau) {
     if (nv <= 256) l.go<64>(logprob_fwd_k<BF, 64, S>, logits, ld, labels, logp, lse, coef, vocab, ignore_index, inv_tau);
-    else if (nv <= 2048) l.go<256>(logprob_fwd_k<BF, 256, S>, logits, ld, labels, logp, lse, coef, vocab, ignore_index, inv_tau);
-    else if (l.rows >= 512) l.go<512>(logprob_fwd_k<BF, 512, S>, logits, ld, labels, logp, lse, coef, vocab, ignore_index, inv_tau);
+    else if (nv <= 4096 && (l.rows >= 512 || nv <= 1024)) l.go<256>(logprob_fwd_k<BF, 256, S>, logits, ld, labels, logp, lse, coef, vocab, ignore_index, inv_tau);
     else l.go<1024>(logprob_fwd_k<BF, 1024, S>, logits, ld, labels, logp, lse, coef, vocab, ignore_index, inv_tau);
 }
 
+// Backward, 16 384 x 92 544 bf16: 256 threads with 4 loads in flight 930 us, 512 x 4 916, 1024 x 4 882, 1024 x 8 871, 1024 x 12 891; 4000 x 10 001 bf16: 256 x 4 36, 1024 x 4 40.
 template <bool BF, bool S>
 void launch_bwd(const Launch& l, int nv, const void* logits, int64_t ld, void* dlogits, int64_t ldd, const int64_t* labels, const float* lse, const float* coef, const float* dloss,
                 float dloss_mul, int vocab, int64_t ignore_index, double inv_tau) {
     if (nv <= 256) l.go<64>(logprob_bwd_k<BF, 64, 4, S>, logits, ld, dlogits, ldd, labels, lse, coef, dloss, dloss_mul, vocab, ignore_index, inv_tau);
     else if (nv <= 2048) l.go<256>(logprob_bwd_k<BF, 256, 4, S>, logits, ld, dlogits, ldd, labels, lse, coef, dloss, dloss_mul, vocab, ignore_index, inv_tau);
-    else l.go<1024>(logprob_bwd_k<BF, 1024, 4, S>, logits, ld, dlogits, ldd, labels, lse, coef, dloss, dloss_mul, vocab, ignore_index, inv_tau);
+    else l.go<1024>(logprob_bwd_k<BF, 1024, 8, S>, logits, ld, dlogits, ldd, labels, lse, coef, dloss, dloss_mul, vocab, ignore_index, inv_tau);
 }
 
-// threads and vectors a thread of the fused kernel: the smallest that hold the row
-inline int fused_threads(int nv) { return nv <= 256 ? 64 : nv <= 2048 ? 256 : 1024; }
+// Threads and vectors a thread of the fused kernel: what the row fills at least half.  16 384 x 92 544 bf16: 1024 x 12 967 us, 1024 x 16 985, reading again (0) 1003;
+// 8192 x 32 000: 512 x 8 160, 1024 x 8 170, 0 169; 8000 x 16 000: 256 x 8 93, 512 x 8 98, 0 113; 8000 x 4000: 256 x 4 26, 0 34.
+inline int fused_threads(int nv) { return nv <= 256 ? 64 : nv <= 2048 ? 256 : nv <= 4096 ? 512 : 1024; }
 
 template <bool BF, bool S>
 void launch_fused(const Launch& l, int nv, const PolicyArgs& a, const void* logits, int64_t ld, void* dlogits, int64_t ldd, float* logp, float* lse, const float* dloss, float dloss_mul,
                   double inv_tau) {
-    if (nv <= 256) l.go<64>(policy_fused_k<BF, 64, 4, S>, a, logits, ld, dlogits, ldd, logp, lse, dloss, dloss_mul, inv_tau);
-    else if (nv <= 2048) l.go<256>(policy_fused_k<BF, 256, 8, S>, a, logits, ld, dlogits, ldd, logp, lse, dloss, dloss_mul, inv_tau);
-    else if (nv <= 4096) l.go<1024>(policy_fused_k<BF, 1024, 4, S>, a, logits, ld, dlogits, ldd, logp, lse, dloss, dloss_mul, inv_tau);
-    else if (nv <= 8192) l.go<1024>(policy_fused_k<BF, 1024, 8, S>, a, logits, ld, dlogits, ldd, logp, lse, dloss, dloss_mul, inv_tau);
-    else if (nv <= 12288) l.go<1024>(policy_fused_k<BF, 1024, 12, S>, a, logits, ld, dlogits, ldd, logp, lse, dloss, dloss_mul, inv_tau);
-    else if (nv <= 16384) l.go<1024>(policy_fused_k<BF, 1024, 16, S>, a, logits, ld, dlogits, ldd, logp, lse, dloss, dloss_mul, inv_tau);
-    else l.go<1024>(policy_fused_k<BF, 1024, 0, S>, a, logits, ld, dlogits, ldd, logp, lse, dloss, dloss_mul, inv_tau);
+    if (nv <= 128) l.go<64>(policy_fused_k<BF, 64, 2, true, S>, a, logits, ld, dlogits, ldd, logp, lse, dloss, dloss_mul, inv_tau);
+    else if (nv <= 256) l.go<64>(policy_fused_k<BF, 64, 4, true, S>, a, logits, ld, dlogits, ldd, logp, lse, dloss, dloss_mul, inv_tau);
+    else if (nv <= 1024) l.go<256>(policy_fused_k<BF, 256, 4, true, S>, a, logits, ld, dlogits, ldd, logp, lse, dloss, dloss_mul, inv_tau);
+    else if (nv <= 2048) l.go<256>(policy_fused_k<BF, 256, 8, true, S>, a, logits, ld, dlogits, ldd, logp, lse, dloss, dloss_mul, inv_tau);
+    else if (nv <= 4096) l.go<512>(policy_fused_k<BF, 512, 8, true, S>, a, logits, ld, dlogits, ldd, logp, lse, dloss, dloss_mul, inv_tau);
+    else if (nv <= 8192) l.go<1024>(policy_fused_k<BF, 1024, 8, true, S>, a, logits, ld, dlogits, ldd, logp, lse, dloss, dloss_mul, inv_tau);
+    else if (nv <= 12288) l.go<1024>(policy_fused_k<BF, 1024, 12, false, S>, a, logits, ld, dlogits, ldd, logp, lse, dloss, dloss_mul, inv_tau);
+    else if (nv <= 16384) l.go<1024>(policy_fused_k<BF, 1024, 16, false, S>, a, logits, ld, dlogits, ldd, logp, lse, dloss, dloss_mul, inv_tau);
+    else l.go<1024>(policy_fused_k<BF, 1024, 0, false, S>, a, logits, ld, dlogits, ldd, logp, lse, dloss, dloss_mul, inv_tau);
 }
 
 // fn<type, stream>(args...)
