@@ -12,6 +12,8 @@
 
 #include <math.h>
 
+#include <algorithm>
+
 namespace {
 
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
@@ -245,9 +247,9 @@ __device__ __forceinline__ void row_zero(typename Elem<BF>::T* d, int vocab) {
 // coef (may be null) is cleared: the loss kernels behind this one set it for the rows of their sequences only.
 template <bool BF, int NT, bool S>
 __global__ __launch_bounds__(NT) void logprob_fwd_k(const void* __restrict__ logits, int64_t ld, const int64_t* __restrict__ labels, float* __restrict__ logp,
-                                                    float* __restrict__ lse, float* __restrict__ coef, int vocab, int64_t ignore_index, double inv_tau) {
+                                                    float* __restrict__ lse, float* __restrict__ coef, int vocab, int64_t ignore_index, double inv_tau, int64_t row0) {
     __shared__ float sh[NT / 32];
-    const int64_t row = blockIdx.x;
+    const int64_t row = row0 + blockIdx.x;
     int lab;
     if (!row_label(labels, row, ignore_index, vocab, lab)) {
         if (threadIdx.x == 0) { logp[row] = 0.f; lse[row] = 0.f; if (coef) coef[row] = 0.f; }
@@ -264,33 +266,55 @@ __global__ __launch_bounds__(NT) void logprob_fwd_k(const void* __restrict__ log
     }
 }
 
-template <bool BF, int NT, int U, bool S>
+// `parts` workgroups a row, one vector a thread and no loop: the chip's reads and writes then move through memory as one dense front, which HBM serves at 6.6 TB/s of
+// mixed traffic where workgroups that walk a row each get 5.5.  16 384 x 92 544 bf16, 40 % masked: 785 us (a workgroup a row: 871).
+template <bool BF, int NT, bool S>
 __global__ __launch_bounds__(NT) void logprob_bwd_k(const void* logits, int64_t ld, void* dlogits, int64_t ldd, const int64_t* __restrict__ labels,
                                                     const float* __restrict__ lse, const float* __restrict__ coef, const float* __restrict__ dloss, float dloss_mul,
-                                                    int vocab, int64_t ignore_index, double inv_tau) {
+                                                    int vocab, int64_t ignore_index, double inv_tau, double log2e, int64_t row0, int parts) {
+    typedef typename Elem<BF>::T T;
+    constexpr int N = Elem<BF>::N;
     __shared__ float sh[NT / 32];
-    const int64_t row = blockIdx.x;
+    const int64_t row = row0 + blockIdx.x / parts;
+    const int part = blockIdx.x % parts, nv = vocab / N, i = part * NT + threadIdx.x;
+    T* d = (T*)dlogits + row * ldd;
+    const T* x = (const T*)logits + row * ld;
     int lab;
-    typename Elem<BF>::T* d = (typename Elem<BF>::T*)dlogits + row * ldd;
     const bool valid = row_label(labels, row, ignore_index, vocab, lab);
     float g = valid ? coef[row] * dloss_mul * (float)inv_tau : 0.f;
     if (dloss) g *= dloss[0];
-    if (!valid || g == 0.f) { row_zero<BF, NT, S>(d, vocab); return; }
-    const float k = (float)(inv_tau * kLog2e);
-    const typename Elem<BF>::T* x = (const typename Elem<BF>::T*)logits + row * ld;
-    const float xl = Elem<BF>::get(x + lab);
-    // p = 2^(x k - l k), l = lse tau: what rounding l k to 32 bits loses goes into the factor
-    const double l = (double)lse[row] / inv_tau * (double)k;
-    const float r = (float)l;
-    if (fabsf(r) <= kRange) {
-        const float g_p = g * exp2_((float)((double)r - l));
-        __syncthreads();   // xl is read before another wave's stores may replace it
-        row_grad<BF, NT, U, S, true>(x, d, vocab, k, r, g, g_p, lab, xl);
-    } else {   // out of the fast form's range, where the log-sum-exp cannot hold the sum beside the maximum
-        const RowStat st = row_stat<BF, NT, 4, S>(x, vocab, k, sh);
-        __syncthreads();
-        row_grad_again<BF, NT>(x, d, vocab, k, st.r, g, g / st.s, lab, xl);
+    const int e = part == parts - 1 ? nv * N + (int)threadIdx.x : vocab;   // the row's last elements, fewer than a vector
+    if (!valid || g == 0.f) {
+        if (i < nv) stv<S>(d + (int64_t)i * N, u32x4{0, 0, 0, 0});
+        if (e < vocab) Elem<BF>::put(d + e, 0.f);
+        return;
     }
+    // p = 2^(x k - l), l = lse log2(e): what rounding l to 32 bits loses goes into the factor
+    const float k = (float)(inv_tau * kLog2e);
+    const double l = (double)lse[row] * log2e;
+    const float r = (float)l;
+    if (!(fabsf(r) <= kRange)) {   // out of the fast form's range, where the log-sum-exp cannot hold the sum beside the maximum: one workgroup for the whole row
+        if (part != 0) return;
+        const float xl = Elem<BF>::get(x + lab);
+        const RowStat st = row_stat<BF, NT, 4, S>(x, vocab, k, sh);
+        __syncthreads();           // the row is read before any store may replace it
+        row_grad_again<BF, NT>(x, d, vocab, k, st.r, g, g / st.s, lab, xl);
+        return;
+    }
+    const float g_p = g * exp2_((float)((double)r - l));
+    if (i < nv) {
+        const u32x4 w = ldv<S>(x + (int64_t)i * N);
+        float v[N];
+        Elem<BF>::unpack(w, v);
+#pragma unroll
+        for (int q = 0; q < N; ++q) v[q] = -g_p * term<true>(v[q], k, r);
+        if ((unsigned)(lab - i * N) < (unsigned)N) {
+#pragma unroll
+            for (int q = 0; q < N; ++q) v[q] += i * N + q == lab ? g : 0.f;
+        }
+        stv<S>(d + (int64_t)i * N, Elem<BF>::pack(v));
+    }
+    if (e < vocab) Elem<BF>::put(d + e, (e == lab ? g : 0.f) - g_p * term<true>(Elem<BF>::get(x + e), k, r));
 }
 
 // ------------------------------------------------------------------------------------------ sums over a workgroup in 64 bits, fixed order
@@ -311,8 +335,6 @@ __device__ __forceinline__ void seq_range(const int32_t* cu, int64_t s, int64_t 
     begin = min(max((int64_t)cu[s], (int64_t)0), rows);
     end = min(max((int64_t)cu[s + 1], begin), rows);
 }
-
-constexpr int kSmallRows = 4096;   // rows that one workgroup finishes alone after their log-probabilities
 
 // ------------------------------------------------------------------------------------------ preference loss
 struct PrefArgs {
@@ -354,80 +376,100 @@ __device__ __forceinline__ bool pref_label(const PrefRows& p, int64_t t) {
     return row_label(p.labels, t, p.ignore_index, p.vocab, lab);
 }
 
-// Sequences 2i, 2i + 1 by NT threads: sums of the log-probabilities in 64 bits, the pair's loss (returned to every thread), the coefficient of every row of the pair.
-// NT = 64: the calling wave; otherwise the workgroup (scratch: NT / 64 doubles).
-template <int NT>
-__device__ __forceinline__ double preference_pair(const PrefRows& r, const PrefArgs& a, int64_t i, double* scratch) {
-    const int tid = threadIdx.x & (NT - 1);
-    int64_t begin[2], end[2];
-    double l[2], n[2];
-#pragma unroll
-    for (int c = 0; c < 2; ++c) {
-        seq_range(r.cu, 2 * i + c, r.rows, begin[c], end[c]);
-        l[c] = 0.0;
-        int cnt = 0;
+// Sequence s by G waves, of which this is number `sub`: the wave's share of its rows' log-probabilities, summed in 64 bits (masked rows hold 0), and of their number.
+template <int G>
+__device__ __forceinline__ void pref_sums(const PrefRows& r, int64_t s, int sub, double& sum, double& cnt) {
+    int64_t begin, end;
+    seq_range(r.cu, s, r.rows, begin, end);
+    double l = 0.0;
+    int n = 0;
 #pragma unroll 4
-        for (int64_t t = begin[c] + tid; t < end[c]; t += NT)
-            if (pref_label(r, t)) { l[c] += (double)r.logp[t]; ++cnt; }
-        n[c] = (double)cnt;
+    for (int64_t t = begin + sub * 64 + (threadIdx.x & 63); t < end; t += G * 64) {
+        l += (double)r.logp[t];
+        n += pref_label(r, t) ? 1 : 0;
     }
+    sum = wave_sum_d(l);
+    cnt = wave_sum_d((double)n);
+}
+
+// the pair that sequence s belongs to, from its two sums and counts: its loss and d loss / d logp of a row of s
+__device__ __forceinline__ double pref_pair(const PrefRows& r, const PrefArgs& a, int64_t s, double l[2], double n[2], bool write, float& w) {
     double gain[2];
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
-        l[c] = NT == 64 ? wave_sum_d(l[c]) : block_sum_d<NT / 64>(l[c], scratch);
-        n[c] = fmax(NT == 64 ? wave_sum_d(n[c]) : block_sum_d<NT / 64>(n[c], scratch), 1.0);
+        const int64_t q = (s & ~(int64_t)1) + c;
+        n[c] = fmax(n[c], 1.0);
         if (a.average) l[c] /= n[c];
-        gain[c] = l[c] - (r.ref ? (double)r.ref[2 * i + c] : 0.0);
-        if (tid == 0) {
-            r.seq_logps[2 * i + c] = (float)l[c];
-            r.rewards[2 * i + c] = (float)(a.beta * gain[c]);
+        gain[c] = l[c] - (r.ref ? (double)r.ref[q] : 0.0);
+        if (write && q == s) {
+            r.seq_logps[s] = (float)l[c];
+            r.rewards[s] = (float)(a.beta * gain[c]);
         }
     }
     double slope;
     const double loss = pair_loss(a, gain[0] - gain[1], slope);
-#pragma unroll
-    for (int c = 0; c < 2; ++c) {
-        const float w = (float)((c ? -slope : slope) / (double)r.pairs / (a.average ? n[c] : 1.0));
-#pragma unroll 4
-        for (int64_t t = begin[c] + tid; t < end[c]; t += NT)
-            if (pref_label(r, t)) r.coef[t] = w;
-    }
+    w = (float)((s & 1 ? -slope : slope) / ((double)r.pairs * (a.average ? n[s & 1] : 1.0)));
     return loss;
 }
 
-__global__ __launch_bounds__(1024) void preference_pair_k(PrefRows r, PrefArgs a, double* __restrict__ losses) {
-    __shared__ double scratch[16];
-    const double loss = preference_pair<1024>(r, a, blockIdx.x, scratch);
-    if (threadIdx.x == 0) losses[blockIdx.x] = loss;
+template <int G>
+__device__ __forceinline__ void pref_coef(const PrefRows& r, int64_t s, int sub, float w) {
+    int64_t begin, end;
+    seq_range(r.cu, s, r.rows, begin, end);
+#pragma unroll 4
+    for (int64_t t = begin + sub * 64 + (threadIdx.x & 63); t < end; t += G * 64)
+        if (pref_label(r, t)) r.coef[t] = w;
+}
+
+// Up to 16 / G sequences, G waves each, in one workgroup: MANY false: the whole batch and its mean loss; true: one pair a workgroup (G = 8), its loss for the mean.
+constexpr int kOnePairs = 8;          // one workgroup finishes a batch of up to this many pairs ...
+constexpr int64_t kOneRows = 32768;   // ... of up to this many rows in all: 16 384 rows, 8 pairs: 14 us, a workgroup a pair and the mean apart 17
+
+template <int G, bool MANY>
+__global__ __launch_bounds__(1024) void preference_pairs_k(PrefRows r, PrefArgs a, float* __restrict__ loss, double* __restrict__ losses) {
+    __shared__ double sum[16], cnt[16], each[kOnePairs];
+    const int w = threadIdx.x >> 6, sub = w % G, first = w / G * G, other = (w / G ^ 1) * G;
+    const int64_t s = (MANY ? 2 * (int64_t)blockIdx.x : 0) + w / G;
+    const bool on = s < 2 * r.pairs;
+    if (on) {
+        double l, n;
+        pref_sums<G>(r, s, sub, l, n);
+        if ((threadIdx.x & 63) == 0) { sum[w] = l; cnt[w] = n; }
+    }
+    __syncthreads();
+    if (on) {
+        double l[2] = {0.0, 0.0}, n[2] = {0.0, 0.0};
+        const int c0 = s & 1 ? other : first, c1 = s & 1 ? first : other;
+        for (int i = 0; i < G; ++i) { l[0] += sum[c0 + i]; n[0] += cnt[c0 + i]; l[1] += sum[c1 + i]; n[1] += cnt[c1 + i]; }
+        float c;
+        const double v = pref_pair(r, a, s, l, n, sub == 0 && (threadIdx.x & 63) == 0, c);
+        if (!(s & 1) && sub == 0 && (threadIdx.x & 63) == 0) {
+            if (MANY) losses[blockIdx.x] = v;
+            else each[s >> 1] = v;
+        }
+        pref_coef<G>(r, s, sub, c);
+    }
+    if (MANY) return;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        double v = 0.0;
+        for (int i = 0; i < (int)r.pairs; ++i) v += each[i];
+        loss[0] = (float)(v / (double)r.pairs);
+    }
 }
 
 __global__ __launch_bounds__(256) void preference_mean_k(const double* __restrict__ losses, int64_t pairs, float* __restrict__ loss) {
     __shared__ double scratch[4];
     double v = 0.0;
+#pragma unroll 4
     for (int64_t i = threadIdx.x; i < pairs; i += 256) v += losses[i];
     v = block_sum_d<4>(v, scratch);
     if (threadIdx.x == 0) loss[0] = (float)(v / (double)pairs);
 }
 
-constexpr int kSmallPairs = 16;   // one workgroup, a wave per pair, finishes a batch of up to this many pairs of up to kSmallRows rows in all
-
-__global__ __launch_bounds__(1024) void preference_small_k(PrefRows r, PrefArgs a, float* __restrict__ loss) {
-    __shared__ double losses[kSmallPairs];
-    const int w = threadIdx.x >> 6;
-    if (w < r.pairs) {
-        const double v = preference_pair<64>(r, a, w, nullptr);
-        if ((threadIdx.x & 63) == 0) losses[w] = v;
-    }
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        double v = 0.0;
-        for (int i = 0; i < (int)r.pairs; ++i) v += losses[i];
-        loss[0] = (float)(v / (double)r.pairs);
-    }
-}
-
 // ------------------------------------------------------------------------------------------ policy loss
 constexpr int kCountRows = 4;      // labels a thread looks at where a row's own workgroup counts
+constexpr int kSmallRows = 4096;
 constexpr int kSmallSeqs = 1024;   // one workgroup finishes a forward pass of up to kSmallRows rows in up to this many sequences
 
 struct PolicyArgs {
@@ -509,7 +551,20 @@ __global__ __launch_bounds__(256) void policy_terms_k(PolicyArgs a, const float*
     if ((threadIdx.x & 63) == 0) a.coef[t] = policy_term(a, policy_row(a, t), (double)logp[t], policy_weight(a, inside, inside ? a.counts[s] : 0), a.terms[t]);
 }
 
-__device__ __forceinline__ void write_stats(const double* v, float kl_coef, float* stats) {
+// sums of the three terms over a workgroup of 1024 threads (scratch: 48 doubles) -> loss, surrogate, KL, clipped share
+__device__ __forceinline__ void write_stats(double* v, float kl_coef, float* stats, double* scratch) {
+#pragma unroll
+    for (int c = 0; c < 3; ++c) {
+        v[c] = wave_sum_d(v[c]);
+        if ((threadIdx.x & 63) == 0) scratch[c * 16 + (threadIdx.x >> 6)] = v[c];
+    }
+    __syncthreads();
+    if (threadIdx.x != 0) return;
+#pragma unroll
+    for (int c = 0; c < 3; ++c) {
+        v[c] = 0.0;
+        for (int w = 0; w < 16; ++w) v[c] += scratch[c * 16 + w];
+    }
     stats[0] = (float)(kl_coef > 0.f ? v[0] + (double)kl_coef * v[1] : v[0]);
     stats[1] = (float)v[0];
     stats[2] = (float)v[1];
@@ -518,12 +573,15 @@ __device__ __forceinline__ void write_stats(const double* v, float kl_coef, floa
 
 // Counts, terms, coefficients and sums of a short batch in one workgroup: a launch less for each, which is all such a call costs.
 __global__ __launch_bounds__(1024) void policy_small_k(PolicyArgs a, const float* __restrict__ logp, float* __restrict__ stats) {
-    __shared__ int cnt[kSmallSeqs];
-    __shared__ double scratch[16];
+    __shared__ int cnt[kSmallSeqs], cu[kSmallSeqs + 1];
+    __shared__ double scratch[48];
     constexpr int R = kSmallRows / 1024;
     int seq[R];   // sequence of each of the thread's rows, -1: no label or outside
     if (a.cu) {
-        for (int i = threadIdx.x; i < a.seqs; i += 1024) cnt[i] = 0;
+        for (int i = threadIdx.x; i <= a.seqs; i += 1024) {
+            cu[i] = a.cu[i];
+            if (i < a.seqs) cnt[i] = 0;
+        }
         __syncthreads();
     }
     int n = 0;
@@ -536,10 +594,10 @@ __global__ __launch_bounds__(1024) void policy_small_k(PolicyArgs a, const float
             int lo = 0, hi = (int)a.seqs;   // how many of cu[1..S] are <= t
             while (lo < hi) {
                 const int mid = (lo + hi) >> 1;
-                if ((int64_t)a.cu[mid + 1] <= t) lo = mid + 1; else hi = mid;
+                if ((int64_t)cu[mid + 1] <= t) lo = mid + 1; else hi = mid;
             }
             int64_t begin = 0, end = 0;
-            if (lo < (int)a.seqs) seq_range(a.cu, lo, a.rows, begin, end);
+            if (lo < (int)a.seqs) seq_range(cu, lo, a.rows, begin, end);
             seq[q] = t >= begin && t < end ? lo : -1;
             if (seq[q] >= 0) atomicAdd(&cnt[lo], 1);   // (whole numbers: the order does not matter)
         }
@@ -556,22 +614,20 @@ __global__ __launch_bounds__(1024) void policy_small_k(PolicyArgs a, const float
         a.coef[t] = seq[q] < 0 ? 0.f : policy_term(a, policy_row(a, t), (double)logp[t], policy_weight(a, true, a.cu ? cnt[seq[q]] : n), term);
         v[0] += (double)term.x; v[1] += (double)term.y; v[2] += (double)term.z;
     }
-    for (int c = 0; c < 3; ++c) v[c] = block_sum_d<16>(v[c], scratch);
-    if (threadIdx.x == 0) write_stats(v, a.kl_coef, stats);
+    write_stats(v, a.kl_coef, stats, scratch);
 }
 
-// Forward and backward of one row: its coefficient needs nothing but the row itself, so the logits are read once.  The row waits in registers, NV
-// vectors a thread (0: longer rows, read again from the last-level cache).  HELD: what waits are its exponentials in 32 bits; otherwise the logits, packed, which are
-// raised a second time.
-template <bool BF, int NT, int NV, bool HELD, bool S>
+// Forward and backward of one row: its coefficient needs nothing but the row itself, so the logits are read once.  NV vectors a thread wait in
+// registers, as exponentials in 32 bits; what a longer row has beyond them (REST) is read again, from the caches.
+template <bool BF, int NT, int NV, bool REST, bool S>
 __global__ __launch_bounds__(NT) void policy_fused_k(PolicyArgs a, const void* logits, int64_t ld, void* dlogits, int64_t ldd, float* __restrict__ logp_out,
-                                                     float* __restrict__ lse_out, const float* __restrict__ dloss, float dloss_mul, double inv_tau) {
+                                                     float* __restrict__ lse_out, const float* __restrict__ dloss, float dloss_mul, double inv_tau, int64_t row0) {
     typedef typename Elem<BF>::T T;
     constexpr int N = Elem<BF>::N;
     __shared__ float sh[NT / 32];
     __shared__ int counted[NT / 64];
     __shared__ float coef_sh;
-    const int64_t row = blockIdx.x;
+    const int64_t row = row0 + blockIdx.x;
     const int vocab = a.vocab;
     T* d = (T*)dlogits + row * ldd;
     int lab;
@@ -601,58 +657,38 @@ __global__ __launch_bounds__(NT) void policy_fused_k(PolicyArgs a, const void* l
     const float xl = Elem<BF>::get(x + lab);
     const float k = (float)(inv_tau * kLog2e);
     const int nv = vocab / N;
-    constexpr int NR = NV > 0 ? NV : 1;
-    u32x4 v[NR];
-    float ex[HELD ? NR * N : 1], ex_rest = 0.f, own = 0.f;   // own: reference of the thread's terms
-    RowStat st;
-    if (NV > 0) {
+    float ex[NV * N], ex_last = -INFINITY;
+    {
+        u32x4 v[NV];
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
             const int i = threadIdx.x + j * NT;
             v[j] = Elem<BF>::ninf();
-            if (i < nv) v[j] = ldv<true>(x + (int64_t)i * N);   // (read once)
+            if (i < nv) v[j] = ldv<true>(x + (int64_t)i * N);
         }
-        float rest = -INFINITY;
-        if (nv * N + (int)threadIdx.x < vocab) rest = Elem<BF>::get(x + nv * N + threadIdx.x);
-        float m = rest;
+        if (nv * N + (int)threadIdx.x < vocab) ex_last = Elem<BF>::get(x + nv * N + threadIdx.x);
 #pragma unroll
-        for (int j = 0; j < NV; ++j) {
-            float e[N];
-            Elem<BF>::unpack(v[j], e);
-#pragma unroll
-            for (int q = 0; q < N; ++q) {
-                m = fmaxf(m, e[q]);
-                if (HELD) ex[j * N + q] = e[q];
-            }
-        }
-        // the vectors stay packed from pass to pass: kept unpacked they would not fit
-        if (!HELD) {
-#pragma unroll
-            for (int j = 0; j < NV; ++j) asm volatile("" : "+v"(v[j]));
-        }
-        own = ref(m, k);
-        float s = ex_rest = term<true>(rest, k, own);
-#pragma unroll
-        for (int j = 0; j < NV; ++j) {
-            float e[N];
-            if (!HELD) Elem<BF>::unpack(v[j], e);
-#pragma unroll
-            for (int q = 0; q < N; ++q) {
-                const float z = term<true>(HELD ? ex[j * N + q] : e[q], k, own);
-                s += z;
-                if (HELD) ex[j * N + q] = z;
-            }
-        }
-        if (!HELD) {
-#pragma unroll
-            for (int j = 0; j < NV; ++j) asm volatile("" : "+v"(v[j]));
-        }
-        st = join_stats<NT>(m, s, k, sh);
-        own = m * k >= -kRange ? exp2_(own - st.r) : 0.f;   // now: the factor of the thread's terms
-        if (!st.fast) st = row_stat_again<BF, NT>(x, vocab, st.m, k, sh);
-    } else {
-        st = row_stat<BF, NT, 4, false>(x, vocab, k, sh);
+        for (int j = 0; j < NV; ++j) Elem<BF>::unpack(v[j], ex + j * N);
     }
+    float m = ex_last, s = 0.f;
+#pragma unroll
+    for (int q = 0; q < NV * N; ++q) m = fmaxf(m, ex[q]);
+    if (REST) {
+        float rm = m;
+        for (int i = NV * NT + threadIdx.x; i < nv; i += NT) {
+            float e[N];
+            Elem<BF>::unpack(ldv<false>(x + (int64_t)i * N), e);
+            add_values<N>(e, k, rm, s);
+        }
+        m = rm;
+    }
+    float own = ref(m, k);   // reference of the thread's terms
+    s += ex_last = term<true>(ex_last, k, own);
+#pragma unroll
+    for (int q = 0; q < NV * N; ++q) s += ex[q] = term<true>(ex[q], k, own);
+    RowStat st = join_stats<NT>(m, s, k, sh);
+    own = m * k >= -kRange ? exp2_(own - st.r) : 0.f;   // now: the factor of the thread's terms
+    if (!st.fast) st = row_stat_again<BF, NT>(x, vocab, st.m, k, sh);
     if (!a.counts) {
 #pragma unroll
         for (int q = 0; q < kCountRows; ++q) n += __popcll(__ballot(live >> q & 1u));
@@ -674,45 +710,38 @@ __global__ __launch_bounds__(NT) void policy_fused_k(PolicyArgs a, const void* l
     const float g_p = g / st.s;
     if (!st.fast) {
         row_grad_again<BF, NT>(x, d, vocab, k, st.r, g, g_p, lab, xl);
-    } else if (NV > 0) {
-        const float f = -g_p * own;
-#pragma unroll
-        for (int j = 0; j < NV; ++j) {
-            const int i = threadIdx.x + j * NT;
-            if (i >= nv) continue;
-            u32x4 out;
-            if (HELD) {
-                float e[N];
-#pragma unroll
-                for (int q = 0; q < N; ++q) e[q] = f * ex[j * N + q];
-                out = Elem<BF>::pack(e);
-            } else {
-                out = grad_vector<BF, true>(v[j], k, st.r, g_p);
-            }
-            stv<S>(d + (int64_t)i * N, out);
-        }
-        if (nv * N + (int)threadIdx.x < vocab) Elem<BF>::put(d + nv * N + threadIdx.x, f * ex_rest);
-        if (owns<BF, NT>(lab, vocab)) Elem<BF>::put(d + lab, g - g_p * term<true>(xl, k, st.r));
-    } else {
-        row_grad<BF, NT, 4, S, true>(x, d, vocab, k, st.r, g, g_p, lab, xl);
+        return;
     }
+    const float f = -g_p * own;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+        const int i = threadIdx.x + j * NT;
+        float e[N];
+#pragma unroll
+        for (int q = 0; q < N; ++q) e[q] = f * ex[j * N + q];
+        if (i < nv) stv<S>(d + (int64_t)i * N, Elem<BF>::pack(e));
+    }
+    if (REST)
+        for (int i = NV * NT + threadIdx.x; i < nv; i += NT) stv<S>(d + (int64_t)i * N, grad_vector<BF, true>(ldv<false>(x + (int64_t)i * N), k, st.r, g_p));
+    if (nv * N + (int)threadIdx.x < vocab) Elem<BF>::put(d + nv * N + threadIdx.x, f * ex_last);
+    if (owns<BF, NT>(lab, vocab)) Elem<BF>::put(d + lab, g - g_p * term<true>(xl, k, st.r));
 }
 
 // stats = {loss, surrogate, KL, clipped share}
 __global__ __launch_bounds__(1024) void policy_stats_k(const float4* __restrict__ terms, int64_t rows, float kl_coef, float* __restrict__ stats) {
-    __shared__ double scratch[16];
+    __shared__ double scratch[48];
     double v[3] = {0.0, 0.0, 0.0};
 #pragma unroll 8
     for (int64_t t = threadIdx.x; t < rows; t += 1024) {
         const float4 q = terms[t];
         v[0] += (double)q.x; v[1] += (double)q.y; v[2] += (double)q.z;
     }
-    for (int c = 0; c < 3; ++c) v[c] = block_sum_d<16>(v[c], scratch);
-    if (threadIdx.x == 0) write_stats(v, kl_coef, stats);
+    write_stats(v, kl_coef, stats, scratch);
 }
 
 constexpr int64_t kMaxVocab = int64_t(1) << 30;   // in-row indices are 32-bit
-constexpr int64_t kMaxRows = 0x7fffffff;          // one workgroup per row
+constexpr int64_t kMaxRows = (int64_t(1) << 26) - 1;   // (a launch of a wave a row has fewer than 2^32 threads)
+constexpr int64_t kMaxSeqs = (int64_t(1) << 22) - 1;   // ... of 1024 threads a sequence
 
 #define IE_CHECK_LOGITS(fn)                                                                                                                              \
     IE_CHECK_ARG(dtype == IE_BF16 || dtype == IE_F32, fn ": bad dtype");                                                                                 \
@@ -732,10 +761,19 @@ bool streams(int64_t rows, int64_t vocab, int dtype) { return rows * vocab * (dt
 
 inline int vectors(int64_t vocab, int dtype) { return (int)(vocab / (dtype == IE_BF16 ? 8 : 4)); }
 
+// rows in slices, so that no launch has 2^32 threads; the kernel's last arguments are the slice's first row, and the workgroups a row if there are several
 struct Launch {
     hipStream_t st;
     int64_t rows;
-    template <int NT, typename F, typename... A> void go(F f, A... args) const { hipLaunchKernelGGL(f, dim3((unsigned)rows), dim3(NT), 0, st, args...); }
+    template <int NT, typename F, typename... A> void go(F f, A... args) const {
+        const int64_t most = (int64_t(1) << 32) / NT - 1;
+        for (int64_t row0 = 0; row0 < rows; row0 += most) hipLaunchKernelGGL(f, dim3((unsigned)std::min(most, rows - row0)), dim3(NT), 0, st, args..., row0);
+    }
+    template <int NT, typename F, typename... A> void parts(F f, int parts, A... args) const {
+        const int64_t most = ((int64_t(1) << 32) / NT - 1) / parts;
+        for (int64_t row0 = 0; row0 < rows; row0 += most)
+            hipLaunchKernelGGL(f, dim3((unsigned)(std::min(most, rows - row0) * parts)), dim3(NT), 0, st, args..., row0, parts);
+    }
 };
 
 // Threads a row.  Forward, 8000 x 4000 bf16: 64 threads 17.3 us, 256 17.8, 512 31; 2000 x 32 000 bf16: 256 22.0, 512 22.6, 1024 24.0; 3001 x 32 003 fp32: 256 54, 512 49,
@@ -747,31 +785,31 @@ void launch_fwd(const Launch& l, int nv, const void* logits, int64_t ld, const i
     else l.go<1024>(logprob_fwd_k<BF, 1024, S>, logits, ld, labels, logp, lse, coef, vocab, ignore_index, inv_tau);
 }
 
-// Backward, 16 384 x 92 544 bf16: 256 threads with 4 loads in flight 930 us, 512 x 4 916, 1024 x 4 882, 1024 x 8 871, 1024 x 12 891; 4000 x 10 001 bf16: 256 x 4 36, 1024 x 4 40.
 template <bool BF, bool S>
 void launch_bwd(const Launch& l, int nv, const void* logits, int64_t ld, void* dlogits, int64_t ldd, const int64_t* labels, const float* lse, const float* coef, const float* dloss,
                 float dloss_mul, int vocab, int64_t ignore_index, double inv_tau) {
-    if (nv <= 256) l.go<64>(logprob_bwd_k<BF, 64, 4, S>, logits, ld, dlogits, ldd, labels, lse, coef, dloss, dloss_mul, vocab, ignore_index, inv_tau);
-    else if (nv <= 2048) l.go<256>(logprob_bwd_k<BF, 256, 4, S>, logits, ld, dlogits, ldd, labels, lse, coef, dloss, dloss_mul, vocab, ignore_index, inv_tau);
-    else l.go<1024>(logprob_bwd_k<BF, 1024, 8, S>, logits, ld, dlogits, ldd, labels, lse, coef, dloss, dloss_mul, vocab, ignore_index, inv_tau);
+    const double log2e = (double)(float)(inv_tau * kLog2e) / inv_tau;   // lse in units of the kernel's x k
+    const int small = (nv + 63) / 64, parts = (nv + 255) / 256;
+    if (nv <= 128) l.parts<64>(logprob_bwd_k<BF, 64, S>, std::max(small, 1), logits, ld, dlogits, ldd, labels, lse, coef, dloss, dloss_mul, vocab, ignore_index, inv_tau, log2e);
+    else l.parts<256>(logprob_bwd_k<BF, 256, S>, parts, logits, ld, dlogits, ldd, labels, lse, coef, dloss, dloss_mul, vocab, ignore_index, inv_tau, log2e);
 }
 
-// Threads and vectors a thread of the fused kernel: what the row fills at least half.  16 384 x 92 544 bf16: 1024 x 12 967 us, 1024 x 16 985, reading again (0) 1003;
-// 8192 x 32 000: 512 x 8 160, 1024 x 8 170, 0 169; 8000 x 16 000: 256 x 8 93, 512 x 8 98, 0 113; 8000 x 4000: 256 x 4 26, 0 34.
-inline int fused_threads(int nv) { return nv <= 256 ? 64 : nv <= 2048 ? 256 : nv <= 4096 ? 512 : 1024; }
+// Threads and vectors a thread of the fused kernel, so that the row fills most of them and two workgroups share a CU while they can.  bf16, rows x vocabulary:
+// 8000 x 4000: 256 x 4 26 us, 64 x 8 27; 8000 x 16 000: 256 x 8 93, 512 x 8 98; 8000 x 20 000: 512 x 8 105, 1024 x 4 156, 256 x 8 + rest 110; 4000 x 50 000:
+// 512 x 10 + rest 141, 1024 x 8 149; 4000 x 60 000: 1024 x 8 180, 512 x 10 + rest 186; 16 384 x 92 544: 1024 x 10 + rest 942, x 8 993, x 12 (spills) 1063, 512 x 10 993.  fp32, 4000 x 92 544: 1024 x 16 + rest 494, x 10 542, x 20 513.
+inline int fused_threads(int nv) { return nv <= 256 ? 64 : nv <= 2048 ? 256 : nv <= 6656 ? 512 : 1024; }
 
 template <bool BF, bool S>
 void launch_fused(const Launch& l, int nv, const PolicyArgs& a, const void* logits, int64_t ld, void* dlogits, int64_t ldd, float* logp, float* lse, const float* dloss, float dloss_mul,
                   double inv_tau) {
-    if (nv <= 128) l.go<64>(policy_fused_k<BF, 64, 2, true, S>, a, logits, ld, dlogits, ldd, logp, lse, dloss, dloss_mul, inv_tau);
-    else if (nv <= 256) l.go<64>(policy_fused_k<BF, 64, 4, true, S>, a, logits, ld, dlogits, ldd, logp, lse, dloss, dloss_mul, inv_tau);
-    else if (nv <= 1024) l.go<256>(policy_fused_k<BF, 256, 4, true, S>, a, logits, ld, dlogits, ldd, logp, lse, dloss, dloss_mul, inv_tau);
-    else if (nv <= 2048) l.go<256>(policy_fused_k<BF, 256, 8, true, S>, a, logits, ld, dlogits, ldd, logp, lse, dloss, dloss_mul, inv_tau);
-    else if (nv <= 4096) l.go<512>(policy_fused_k<BF, 512, 8, true, S>, a, logits, ld, dlogits, ldd, logp, lse, dloss, dloss_mul, inv_tau);
-    else if (nv <= 8192) l.go<1024>(policy_fused_k<BF, 1024, 8, true, S>, a, logits, ld, dlogits, ldd, logp, lse, dloss, dloss_mul, inv_tau);
-    else if (nv <= 12288) l.go<1024>(policy_fused_k<BF, 1024, 12, false, S>, a, logits, ld, dlogits, ldd, logp, lse, dloss, dloss_mul, inv_tau);
-    else if (nv <= 16384) l.go<1024>(policy_fused_k<BF, 1024, 16, false, S>, a, logits, ld, dlogits, ldd, logp, lse, dloss, dloss_mul, inv_tau);
-    else l.go<1024>(policy_fused_k<BF, 1024, 0, false, S>, a, logits, ld, dlogits, ldd, logp, lse, dloss, dloss_mul, inv_tau);
+    if (nv <= 128) l.go<64>(policy_fused_k<BF, 64, 2, false, S>, a, logits, ld, dlogits, ldd, logp, lse, dloss, dloss_mul, inv_tau);
+    else if (nv <= 256) l.go<64>(policy_fused_k<BF, 64, 4, false, S>, a, logits, ld, dlogits, ldd, logp, lse, dloss, dloss_mul, inv_tau);
+    else if (nv <= 1024) l.go<256>(policy_fused_k<BF, 256, 4, false, S>, a, logits, ld, dlogits, ldd, logp, lse, dloss, dloss_mul, inv_tau);
+    else if (nv <= 2048) l.go<256>(policy_fused_k<BF, 256, 8, false, S>, a, logits, ld, dlogits, ldd, logp, lse, dloss, dloss_mul, inv_tau);
+    else if (nv <= 4096) l.go<512>(policy_fused_k<BF, 512, 8, false, S>, a, logits, ld, dlogits, ldd, logp, lse, dloss, dloss_mul, inv_tau);
+    else if (nv <= 6656) l.go<512>(policy_fused_k<BF, 512, 10, true, S>, a, logits, ld, dlogits, ldd, logp, lse, dloss, dloss_mul, inv_tau);
+    else if (nv <= 8192) l.go<1024>(policy_fused_k<BF, 1024, 8, false, S>, a, logits, ld, dlogits, ldd, logp, lse, dloss, dloss_mul, inv_tau);
+    else l.go<1024>(policy_fused_k<BF, 1024, BF ? 10 : 16, true, S>, a, logits, ld, dlogits, ldd, logp, lse, dloss, dloss_mul, inv_tau);
 }
 
 // fn<type, stream>(args...)
@@ -818,7 +856,7 @@ extern "C" int ie_preference_loss_fwd(const void* logits, int dtype, int64_t ld,
                                       void* stream) {
     IE_CHECK_ARG(logits && labels && cu_seqlens && loss && rewards && seq_logps && logp && lse && coef && workspace, "ie_preference_loss_fwd: null pointer");
     IE_CHECK_LOGITS("ie_preference_loss_fwd");
-    IE_CHECK_ARG(pairs > 0 && pairs <= kMaxRows / 2, "ie_preference_loss_fwd: at least one pair");
+    IE_CHECK_ARG(pairs > 0 && pairs <= kMaxSeqs / 2, "ie_preference_loss_fwd: at least one pair");
     IE_CHECK_ARG(kind == IE_PREF_SIGMOID || kind == IE_PREF_HINGE || kind == IE_PREF_IPO, "ie_preference_loss_fwd: unknown kind");
     IE_CHECK_ARG(beta > 0.0 && beta <= 1e30, "ie_preference_loss_fwd: beta must be positive and finite");
     IE_CHECK_ARG(label_smoothing >= 0.0 && label_smoothing <= 0.5 && (kind == IE_PREF_SIGMOID || label_smoothing == 0.0),
@@ -828,11 +866,15 @@ extern "C" int ie_preference_loss_fwd(const void* logits, int dtype, int64_t ld,
     if (rows > 0) IE_ROWS(launch_fwd, logits, ld, labels, logp, lse, coef, (int)vocab, ignore_index, inv_temperature);
     const PrefArgs a = {kind, average, beta, label_smoothing, margin};
     const PrefRows r = {logp, labels, cu_seqlens, ref_logps, rows, pairs, ignore_index, (int)vocab, rewards, seq_logps, coef};
-    if (pairs <= kSmallPairs && rows <= kSmallRows) {
-        hipLaunchKernelGGL(preference_small_k, dim3(1), dim3(1024), 0, st, r, a, loss);
+    double* losses = (double*)workspace;
+    if (pairs <= kOnePairs && rows <= kOneRows) {
+        if (pairs == 1) hipLaunchKernelGGL((preference_pairs_k<8, false>), dim3(1), dim3(1024), 0, st, r, a, loss, losses);
+        else if (pairs == 2) hipLaunchKernelGGL((preference_pairs_k<4, false>), dim3(1), dim3(1024), 0, st, r, a, loss, losses);
+        else if (pairs <= 4) hipLaunchKernelGGL((preference_pairs_k<2, false>), dim3(1), dim3(1024), 0, st, r, a, loss, losses);
+        else hipLaunchKernelGGL((preference_pairs_k<1, false>), dim3(1), dim3(1024), 0, st, r, a, loss, losses);
     } else {
-        hipLaunchKernelGGL(preference_pair_k, dim3((unsigned)pairs), dim3(1024), 0, st, r, a, (double*)workspace);
-        hipLaunchKernelGGL(preference_mean_k, dim3(1), dim3(256), 0, st, (const double*)workspace, pairs, loss);
+        hipLaunchKernelGGL((preference_pairs_k<8, true>), dim3((unsigned)pairs), dim3(1024), 0, st, r, a, loss, losses);
+        hipLaunchKernelGGL(preference_mean_k, dim3(1), dim3(256), 0, st, (const double*)losses, pairs, loss);
     }
     return ie_launch_status("ie_preference_loss_fwd launch");
 }
@@ -850,7 +892,7 @@ extern "C" int ie_policy_loss(const void* logits, int dtype, int64_t ld, void* d
     IE_CHECK_ARG((dlogits != nullptr) == (dloss != nullptr), "ie_policy_loss: dlogits and dloss come together");
     IE_CHECK_ARG(!dlogits || (ldd >= vocab && overlap_ok(logits, ld, dlogits, ldd, rows, vocab, dtype)),
                  "ie_policy_loss: dlogits must be the logits themselves or lie apart from them");
-    IE_CHECK_ARG(cu_seqlens ? seqs > 0 && seqs <= kMaxRows : seqs == 0, "ie_policy_loss: cu_seqlens and the number of sequences come together");
+    IE_CHECK_ARG(cu_seqlens ? seqs > 0 && seqs <= kMaxSeqs : seqs == 0, "ie_policy_loss: cu_seqlens and the number of sequences come together");
     IE_CHECK_ARG(clip_low >= 0.f && clip_low <= 1.f && clip_high >= 0.f && clip_high <= 1e30f, "ie_policy_loss: clip range");
     IE_CHECK_ARG(kl_coef >= 0.f && kl_coef <= 1e30f && (ref_logps || kl_coef == 0.f), "ie_policy_loss: a KL term needs the reference log-probabilities");
     hipStream_t st = (hipStream_t)stream;

@@ -33,8 +33,8 @@ struct ClipList {
     const void* in[kClipTensors];
     void* out[kClipTensors];
     int64_t len[kClipTensors];                   // elements, | kBf | kOutBf
-    int first[kClipTensors + 1];
-    int n, shift;
+    int first[kClipTensors + 1];                 // first workgroup of tensor i
+    int n, u, rounds;                            // a workgroup takes u rounds steps of its threads
 };
 
 // tensor that chunk c belongs to (first[] grows strictly: tensors without elements are not in the table)
@@ -101,19 +101,23 @@ __global__ __launch_bounds__(256) void grad_norm_k(NormList l, double* __restric
 }
 
 // norm from the partial sums, in a fixed order; every thread returns it
+template <int NT>
 __device__ __forceinline__ float join_norm(const double* __restrict__ partial, int n, double* scratch) {
     double acc = 0.0;
 #pragma unroll 4
-    for (int i = threadIdx.x; i < n; i += 256) acc += partial[i];
+    for (int i = threadIdx.x; i < n; i += NT) acc += partial[i];
     acc = wave_sum_d(acc);
     if ((threadIdx.x & 63) == 0) scratch[threadIdx.x >> 6] = acc;
     __syncthreads();
-    return (float)sqrt(scratch[0] + scratch[1] + scratch[2] + scratch[3]);
+    acc = 0.0;
+#pragma unroll
+    for (int w = 0; w < NT / 64; ++w) acc += scratch[w];
+    return (float)sqrt(acc);
 }
 
 __global__ __launch_bounds__(256) void grad_norm_finish_k(const double* __restrict__ partial, int n, float* __restrict__ norm) {
     __shared__ double scratch[4];
-    const float v = join_norm(partial, n, scratch);
+    const float v = join_norm<256>(partial, n, scratch);
     if (threadIdx.x == 0) norm[0] = v;
 }
 
@@ -168,54 +172,85 @@ template <> struct Type<false> {
     static __device__ __forceinline__ T put(float x) { return x; }
 };
 
-template <bool IB, bool OB, bool S>
-__device__ __forceinline__ void chunk_scale(const void* in, void* out, int64_t base, int n, float f) {
-    constexpr int N = IB && OB ? 8 : 4, U = 4;
-    const typename Type<IB>::T* p = (const typename Type<IB>::T*)in + base;
-    typename Type<OB>::T* o = (typename Type<OB>::T*)out + base;
-    const int ns = n / N;
-    auto scale = [&](const Step<IB, N, S>& q, int i) {
+constexpr int kClipThreads = 1024;
+inline __host__ __device__ int step_of(bool in_bf, bool out_bf) { return in_bf && out_bf ? 8 : 4; }
+
+// U rounds of kClipThreads steps, from step `first` of a tensor of n elements on: all loads, then all stores
+template <bool IB, bool OB, int U, bool S>
+__device__ __forceinline__ void scale_steps(const void* in, void* out, int64_t n, int64_t first, float f) {
+    constexpr int N = IB && OB ? 8 : 4;
+    const typename Type<IB>::T* p = (const typename Type<IB>::T*)in;
+    typename Type<OB>::T* o = (typename Type<OB>::T*)out;
+    const int64_t steps = n / N, i = first + threadIdx.x;
+    auto scaled = [&](const Step<IB, N, S>& q, int64_t k) {
         float v[N];
         q.unpack(v);
 #pragma unroll
         for (int e = 0; e < N; ++e) v[e] *= f;
-        Step<OB, N, S>::store(o + i * N, v);
+        Step<OB, N, S>::store(o + k * N, v);
     };
-    int i = threadIdx.x;
-    for (; i + (U - 1) * 256 < ns; i += U * 256) {
+    if (U > 1 && first + U * kClipThreads <= steps) {   // (the same for all threads: no step needs a look at the end)
         Step<IB, N, S> q[U];
 #pragma unroll
-        for (int u = 0; u < U; ++u) q[u].load(p + (i + u * 256) * N);
+        for (int u = 0; u < U; ++u) q[u].load(p + (i + u * kClipThreads) * N);
 #pragma unroll
-        for (int u = 0; u < U; ++u) scale(q[u], i + u * 256);
+        for (int u = 0; u < U; ++u) scaled(q[u], i + u * kClipThreads);
+        return;
     }
-    for (; i < ns; i += 256) {
-        Step<IB, N, S> q;
-        q.load(p + i * N);
-        scale(q, i);
+    for (int u = 0; u < U; ++u) {
+        const int64_t k = i + u * kClipThreads;
+        if (k < steps) {
+            Step<IB, N, S> q;
+            q.load(p + k * N);
+            scaled(q, k);
+        } else if (k - steps < n - steps * N) {   // the elements behind the last whole step, one a thread
+            const int64_t j = steps * N + (k - steps);
+            o[j] = Type<OB>::put(Type<IB>::get(p[j]) * f);
+        }
     }
-    i = ns * N + threadIdx.x;
-    if (i < n) o[i] = Type<OB>::put(Type<IB>::get(p[i]) * f);
 }
 
-// partial sums given: the norm is added up here (and kept by the first workgroup if norm_out is given); otherwise norm holds it
-template <bool S>
-__global__ __launch_bounds__(256) void grad_clip_k(ClipList l, const double* __restrict__ partial, int parts, const float* norm, float* norm_out, double max_norm, int in_place) {
+// min(1, max_norm / (norm + 1e-6)); NaN stays NaN
+__device__ __forceinline__ float clip_factor(float norm, double max_norm) {
+    const double q = max_norm / ((double)norm + 1e-6);
+    return q >= 1.0 ? 1.f : (float)q;
+}
+
+__global__ __launch_bounds__(256) void grad_clip_finish_k(const double* __restrict__ partial, int n, double max_norm, float* __restrict__ norm, float* __restrict__ factor) {
     __shared__ double scratch[4];
-    const float nrm = partial ? join_norm(partial, parts, scratch) : norm[0];
-    if (norm_out && blockIdx.x == 0 && threadIdx.x == 0) norm_out[0] = nrm;
-    const double q = max_norm / ((double)nrm + 1e-6);
-    const float f = q >= 1.0 ? 1.f : (float)q;   // (NaN stays NaN)
-    if (in_place && f == 1.f) return;
-    const int c = blockIdx.x, t = find_tensor(l, c);
-    const int64_t base = (int64_t)(c - l.first[t]) << l.shift, len = l.len[t];
-    const int n = (int)min((len & kLen) - base, (int64_t)1 << l.shift);
-    if (len & kBf) {
-        if (len & kOutBf) chunk_scale<true, true, S>(l.in[t], l.out[t], base, n, f);
-        else chunk_scale<true, false, S>(l.in[t], l.out[t], base, n, f);
+    const float v = join_norm<256>(partial, n, scratch);
+    if (threadIdx.x == 0) { norm[0] = v; factor[0] = clip_factor(v, max_norm); }
+}
+
+// Partial sums given: norm and factor are formed here (and the norm kept by the first workgroup if norm_out is given); otherwise `factor` holds it.
+// What a launch touches at one time should lie close together: HBM then serves mixed reads and writes at 6 TB/s and more.  0.87e9 bf16 gradients into fp32, this kernel
+// alone: 1024 threads with 8 steps each, loads before stores: 862 us; 256 threads with 32 steps, 4 at a time: 953; one step a thread would take 790 but for this
+// kernel's start (table, factor), which makes it 1212.
+template <int U, bool S>
+__global__ __launch_bounds__(kClipThreads) void grad_clip_k(ClipList l, const double* __restrict__ partial, int parts, const float* __restrict__ factor, float* norm_out,
+                                                            double max_norm, int in_place) {
+    __shared__ double scratch[kClipThreads / 64];
+    float f;
+    if (partial) {
+        const float nrm = join_norm<kClipThreads>(partial, parts, scratch);
+        if (norm_out && blockIdx.x == 0 && threadIdx.x == 0) norm_out[0] = nrm;
+        f = clip_factor(nrm, max_norm);
     } else {
-        if (len & kOutBf) chunk_scale<false, true, S>(l.in[t], l.out[t], base, n, f);
-        else chunk_scale<false, false, S>(l.in[t], l.out[t], base, n, f);
+        f = factor[0];
+    }
+    if (in_place && f == 1.f) return;
+    const int t = find_tensor(l, blockIdx.x);
+    const int64_t len = l.len[t], n = len & kLen;
+    const int rounds = l.rounds;   // (1 unless one tensor alone needs more workgroups than a launch has)
+    int64_t first = (int64_t)((int)blockIdx.x - l.first[t]) * rounds * (U * kClipThreads);
+    for (int q = 0; q < rounds; ++q, first += U * kClipThreads) {
+        if (len & kBf) {
+            if (len & kOutBf) scale_steps<true, true, U, S>(l.in[t], l.out[t], n, first, f);
+            else scale_steps<true, false, U, S>(l.in[t], l.out[t], n, first, f);
+        } else {
+            if (len & kOutBf) scale_steps<false, true, U, S>(l.in[t], l.out[t], n, first, f);
+            else scale_steps<false, false, U, S>(l.in[t], l.out[t], n, first, f);
+        }
     }
 }
 
@@ -250,22 +285,32 @@ int check_list(const char* msg, Lists& l) {
     return IE_OK;
 }
 
+inline int64_t blocks_of(const NormList& t, const Lists& l, int64_t i) { return (l.numels[i] + (int64_t(1) << t.shift) - 1) >> t.shift; }
+inline int64_t blocks_of(const ClipList& t, const Lists& l, int64_t i) {
+    const bool in = l.dtypes[i] == IE_BF16, out = l.outs ? l.out_dtypes[i] == IE_BF16 : in;
+    const int64_t steps = l.numels[i] / step_of(in, out) + l.numels[i] % step_of(in, out), per = (int64_t)kClipThreads * t.u * t.rounds;   // (whole steps, then elements)
+    return (steps + per - 1) / per;
+}
+inline void longer(NormList& t) { ++t.shift; }
+inline void longer(ClipList& t) { t.rounds *= 2; }
 inline void put_out(NormList&, int, const Lists&, int64_t) {}
 inline void put_out(ClipList& t, int k, const Lists& l, int64_t i) {
     t.out[k] = l.outs ? l.outs[i] : (void*)l.ptrs[i];
     if ((l.outs ? l.out_dtypes[i] : l.dtypes[i]) == IE_BF16) t.len[k] |= kOutBf;
 }
 
-// the next launch's tensors, from i on; returns where the one after it starts.  (2^38 elements are 2^23 chunks at the largest chunk: one tensor always fits.)
+// the next launch's tensors, from i on; returns where the one after it starts.  A launch has fewer than 2^22 workgroups (2^32 threads); a tensor that needs more of them
+// alone gets longer chunks.
 template <int CAP, typename L>
 int64_t fill(L& t, int64_t i, const Lists& l) {
+    constexpr int64_t most = (int64_t(1) << 22) - 1;
     t.n = 0;
-    t.shift = l.shift;
     int64_t total = 0;
     for (; i < l.n && t.n < CAP; ++i) {
         if (l.numels[i] == 0) continue;
-        const int64_t chunks = (l.numels[i] + (int64_t(1) << l.shift) - 1) >> l.shift;
-        if (total + chunks > (int64_t(1) << 30)) break;
+        while (t.n == 0 && blocks_of(t, l, i) > most) longer(t);
+        const int64_t chunks = blocks_of(t, l, i);
+        if (total + chunks > most) break;
         t.in[t.n] = l.ptrs[i];
         t.len[t.n] = l.numels[i] | (l.dtypes[i] == IE_BF16 ? kBf : 0);
         put_out(t, t.n, l, i);
@@ -281,6 +326,7 @@ int launch_norm(const Lists& l, double* partial, hipStream_t st) {
     NormList t;
     int used = 0;
     for (int64_t i = 0; i < l.n;) {
+        t.shift = l.shift;
         i = fill<kNormTensors>(t, i, l);
         if (t.n == 0) continue;
         const int blocks = std::min(t.first[t.n], kNormBlocks);
@@ -323,7 +369,7 @@ int check_overlap(const Lists& l) {
 
 }  // namespace
 
-extern "C" int64_t ie_grad_norm_workspace(int64_t n) { return n < 0 ? 0 : (n / kNormTensors + 1) * kNormBlocks * 8; }
+extern "C" int64_t ie_grad_norm_workspace(int64_t n) { return n < 0 ? 0 : (n / kNormTensors + 1) * kNormBlocks * 8 + 8; }
 
 extern "C" int ie_grad_norm(const void* const* ptrs, const int64_t* numels, const int* dtypes, int64_t n, void* workspace, float* norm, void* stream) {
     IE_CHECK_ARG(workspace && norm, "ie_grad_norm: null pointer");
@@ -346,19 +392,29 @@ extern "C" int ie_grad_clip(const void* const* ptrs, const int64_t* numels, cons
     rc = check_overlap(l);
     if (rc != IE_OK) return rc;
     hipStream_t st = (hipStream_t)stream;
-    const double* partial = (const double*)workspace;
-    const int parts = launch_norm(l, (double*)workspace, st);
+    double* partial = (double*)workspace;
+    const int parts = launch_norm(l, partial, st);
     const bool joined = parts <= kJoined && parts > 0;
-    if (!joined) hipLaunchKernelGGL(grad_norm_finish_k, dim3(1), dim3(256), 0, st, partial, parts, norm);
+    float* factor = (float*)(partial + ie_grad_norm_workspace(n) / 8 - 1);   // behind the partial sums
+    if (!joined) hipLaunchKernelGGL(grad_clip_finish_k, dim3(1), dim3(256), 0, st, (const double*)partial, parts, max_norm, norm, factor);
     ClipList t;
     float* norm_out = joined ? norm : nullptr;
+    const double* from = joined ? partial : nullptr;
     for (int64_t i = 0; i < n;) {
+        // 8 steps a thread where they leave every CU at least 4 workgroups
+        t.u = l.elems >= int64_t(8) * 4 * kClipThreads * 1024 ? 8 : 1;
+        t.rounds = 1;
         i = fill<kClipTensors>(t, i, l);
         if (t.n == 0) continue;
         const dim3 grid((unsigned)t.first[t.n]);
-        const double* from = joined ? partial : nullptr;
-        if (l.stream) hipLaunchKernelGGL((grad_clip_k<true>), grid, dim3(256), 0, st, t, from, parts, (const float*)norm, norm_out, max_norm, (int)(outs == nullptr));
-        else hipLaunchKernelGGL((grad_clip_k<false>), grid, dim3(256), 0, st, t, from, parts, (const float*)norm, norm_out, max_norm, (int)(outs == nullptr));
+        const int in_place = outs == nullptr;
+        if (t.u == 8) {
+            if (l.stream) hipLaunchKernelGGL((grad_clip_k<8, true>), grid, dim3(kClipThreads), 0, st, t, from, parts, (const float*)factor, norm_out, max_norm, in_place);
+            else hipLaunchKernelGGL((grad_clip_k<8, false>), grid, dim3(kClipThreads), 0, st, t, from, parts, (const float*)factor, norm_out, max_norm, in_place);
+        } else {
+            if (l.stream) hipLaunchKernelGGL((grad_clip_k<1, true>), grid, dim3(kClipThreads), 0, st, t, from, parts, (const float*)factor, norm_out, max_norm, in_place);
+            else hipLaunchKernelGGL((grad_clip_k<1, false>), grid, dim3(kClipThreads), 0, st, t, from, parts, (const float*)factor, norm_out, max_norm, in_place);
+        }
         norm_out = nullptr;
     }
     return ie_launch_status("ie_grad_clip launch");

@@ -317,6 +317,62 @@ def test_policy_loss(dev, rows, V, cu, kl, dtype):
     assert d3.data_ptr() == x3.data_ptr() and torch.equal(d3, d2) and torch.equal(b3.stats, b.stats)
 
 
+@pytest.mark.parametrize("dtype", DTYPES, ids=["bf16", "fp32"])
+@pytest.mark.parametrize("rows, V", SIZES + [(3, 9001), (2, 17001), (3, 45001), (2, 60007), (2, 70001)])
+def test_policy_loss_in_one_pass_at_every_row_length(dev, rows, V, dtype):
+    """Rows of every length class of the one-pass kernel (held whole, held in part, a rest behind the last whole vector), in place and apart, aligned and not."""
+    for pad, shift, mask in ((0, 0, 0.0), (5, 1, 0.3)):
+        x, y = make(dev, rows, V, dtype, rows * 31 + V, pad, shift, mask)
+        old, adv, ref = policy_inputs(dev, x, y, V, 0.2, 0.2)
+        dloss = torch.full((1,), 16.0, device=dev)
+        before = x.clone()
+        b, d = K().policy_loss_fwd_bwd(x, y, old, adv, dloss, dlogits=torch.full_like(x, 7.0), ref_logps=ref, kl_coef=0.1)
+        lp, ls, valid, z = ref_logp(x, y)
+        check(b.logp, lp, lp_tol(V, z), "logp")
+        check(b.lse, ls, lp_tol(V, z) + U * ls.abs(), "lse")
+        stats, coef, tol, kl_tol = policy_ref(b.logp, y, old, adv, ref, 0.2, 0.2, 0.1, None)
+        check(b.coef, coef, tol, "coef")
+        check_dlogits(d, x, y, b.coef.double() * 16.0, "dlogits")
+        assert torch.equal(x, before)
+        flat = torch.full((rows, V + 3), 5.0, dtype=dtype, device=dev)
+        flat[:, :V] = x
+        b2, d2 = K().policy_loss_fwd_bwd(flat[:, :V], y, old, adv, dloss, ref_logps=ref, kl_coef=0.1)
+        assert torch.equal(flat[:, :V], d) and torch.equal(b2.stats, b.stats) and bool((flat[:, V:] == 5.0).all())
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=["bf16", "fp32"])
+@pytest.mark.parametrize("V", [3000, 60007, 92544])
+def test_policy_loss_in_one_pass_with_infinite_and_lowest_logits(dev, dtype, V):
+    """The rows of test_infinite_and_nan_logits_in_live_rows through the one-pass kernel: forbidden by -inf or by the type's lowest value, in part and as a whole."""
+    x, y = make(dev, 6, V, dtype, 3, mask=0.0)
+    y[:] = torch.arange(6, device=dev) * 300 + 5
+    lowest = torch.finfo(dtype).min
+    x[0, 7:2900] = -math.inf
+    x[1] = lowest; x[1, 305] = 1.0
+    x[2] = lowest                              # uniform at the lowest value
+    x[3, 11] = math.nan
+    x[4, 1205] = 300.0
+    x[5, :] = -math.inf; x[5, 1505] = -2.0; x[5, 7] = -3.0
+    zero, one = torch.zeros(6, device=dev), torch.ones(1, device=dev)
+    want = K().token_logprobs(x, y)[0]
+    old = torch.where(want.isnan(), zero, want)
+    b, d = K().policy_loss_fwd_bwd(x, y, old, zero + 1.0, one, dlogits=torch.empty_like(x))
+    f = K().policy_loss_fwd(x, y, old, zero + 1.0)
+    e = K().policy_loss_bwd(x, y, f, one, dlogits=torch.empty_like(x))
+    assert bool(b.logp[3].isnan()) and bool(d[3].isnan().all()) and bool(e[3].isnan().all())
+    assert abs(float(b.logp[2]) + math.log(V)) <= lp_tol(V, torch.tensor([8.0]))
+    sel = [0, 1, 4, 5]
+    lp, ls, valid, z = ref_logp(x[sel], y[sel])
+    check(b.logp[sel], lp, lp_tol(V, z), "logp")
+    for got, r in ((d, b), (e, f)):
+        check_dlogits(got[sel], x[sel], y[sel], r.coef[sel].double(), "dlogits")
+        p = torch.full((V,), 1.0 / V, dtype=torch.float64)
+        hot = torch.zeros(V, dtype=torch.float64)
+        hot[605] = 1.0
+        c = float(r.coef[2])
+        check(got[2], c * (hot - p), (torch.finfo(dtype).eps / 2 + 16 * U) * abs(c) * (hot + p), "uniform row")
+
+
 def test_policy_loss_without_a_token(dev):
     x, _ = make(dev, 6, 100, torch.bfloat16, 1)
     y = torch.full((6,), IGNORE, device=dev)
