@@ -226,15 +226,17 @@ def prepare(case, seed):
 
 # ------------------------------------------------------------------------------------------------ plain forms
 def _plain_softmax(logits, labels, temperature):
+    """Log-probabilities and log-sum-exps, valid rows, exponentials and their sums.  Long sums and their logarithms are in 64 bits: a log-probability is the small difference of
+    two numbers near 20, and a sequence adds up hundreds of them."""
     z = logits.float() / temperature
     m = z.amax(1, keepdim=True)
     e = torch.exp(z - m)
-    s = e.sum(1, keepdim=True)
-    lse = (m + torch.log(s))[:, 0]
+    s = e.sum(1, keepdim=True, dtype=torch.float64)
+    log_s = torch.log(s)[:, 0]
     valid = labels >= 0
-    logp = z.gather(1, labels.clamp(min=0)[:, None])[:, 0] - lse
-    zero = torch.zeros_like(lse)
-    return torch.where(valid, logp, zero), torch.where(valid, lse, zero), valid, e, s
+    logp = (z.gather(1, labels.clamp(min=0)[:, None]) - m)[:, 0].double() - log_s
+    zero = torch.zeros_like(log_s)
+    return torch.where(valid, logp, zero), torch.where(valid, m[:, 0].double() + log_s, zero), valid, e, s.float()
 
 
 def _plain_dlogits(logits, labels, valid, e, s, dlogp, temperature):
@@ -254,7 +256,7 @@ def _plain_preference(st):
     seq = torch.bucketize(torch.arange(c["tokens"], device=logp.device, dtype=torch.int32), st["cu"], right=True, out_int32=True).long() - 1
     inside = valid & (seq < n)
     seq = seq.clamp(max=n - 1)
-    total = torch.zeros(n, dtype=torch.float64, device=logp.device).index_add_(0, seq, (logp * inside).double())
+    total = torch.zeros(n, dtype=torch.float64, device=logp.device).index_add_(0, seq, logp * inside)
     count = torch.zeros(n, dtype=torch.float64, device=logp.device).index_add_(0, seq, inside.double())
     if c["average"]:
         total = total / count.clamp(min=1)
@@ -284,7 +286,7 @@ def _plain_preference(st):
 def _plain_policy(st):
     c = st["case"]
     logp, lse, valid, e, s = _plain_softmax(st["logits"], st["labels"], c["temperature"])
-    zero = torch.zeros_like(logp)
+    zero = torch.zeros_like(logp, dtype=torch.float32)
     if c["by_sequence"]:
         n = c["seqs"]
         seq = torch.bucketize(torch.arange(c["tokens"], device=logp.device, dtype=torch.int32), st["cu"], right=True, out_int32=True).long() - 1
@@ -295,19 +297,19 @@ def _plain_policy(st):
     else:
         w = valid.float() / valid.float().sum().clamp(min=1)
     adv = torch.where(valid, st["adv"], zero)
-    ratio = torch.exp(torch.where(valid, logp - st["old"], zero))
+    ratio = torch.exp(torch.where(valid, (logp - st["old"]).float(), zero))
     low, high = 1 - c["low"], 1 + c["high"]
     clipped = ((adv > 0) & (ratio > high)) | ((adv < 0) & (ratio < low))
     surrogate = -torch.minimum(ratio * adv, ratio.clamp(low, high) * adv)
     dlogp = torch.where(clipped, zero, -ratio * adv)
     kl = zero
     if c["kl"] > 0:
-        d = torch.where(valid, st["ref"] - logp, zero)
+        d = torch.where(valid, (st["ref"] - logp).float(), zero)
         kl = torch.exp(d) - d - 1
         dlogp = dlogp + c["kl"] * (1 - torch.exp(d))
     sums = [(w.double() * t.double()).sum() for t in (surrogate, kl, clipped)]
     stats = torch.stack([sums[0] + c["kl"] * sums[1], *sums]).float()
-    out = [stats, logp]
+    out = [stats, logp.float()]
     if c["form"] != "forward":
         out.append(_plain_dlogits(st["logits"], st["labels"], valid, e, s, dlogp * w * st["dloss"], c["temperature"]))
     return out
@@ -332,7 +334,7 @@ def run(st):
     c = st["case"]
     if not own:
         if c["op"] == "logprobs":
-            return list(_plain_softmax(st["logits"], st["labels"], c["temperature"])[:2])
+            return [t.float() for t in _plain_softmax(st["logits"], st["labels"], c["temperature"])[:2]]
         return {"preference": _plain_preference, "policy": _plain_policy, "clip": _plain_clip}[c["op"]](st)
     from internevo_amd import kernels as K
 
