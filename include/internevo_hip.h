@@ -506,7 +506,7 @@ int ie_gemm_set_wgrad_ksplit_workspace(void* ws, int64_t bytes);
  *     IE_PREF_HINGE    max(0, 1 - z)
  *     IE_PREF_IPO      (h - 1 / (2 beta))^2                          (no margin)
  *   loss[0] = mean over the pairs; rewards [2 pairs] = beta (l - ref); seq_logps [2 pairs] = l; coef [rows] = d loss / d logp for ie_logprob_bwd.
- *   Sums and losses are formed in 64 bits.  workspace: ie_preference_loss_workspace(pairs) bytes, 8-byte aligned, for this call only.
+ *   Sums and losses are formed in 64 bits, from log-probabilities that are not rounded to 32 first.  workspace: ie_preference_loss_workspace(rows, pairs) bytes, 8-byte aligned, for this call only.
  *
  * ie_policy_loss: r = exp(logp - old_logps), loss term -min(r A, clamp(r, 1 - clip_low, 1 + clip_high) A) + kl_coef (exp(q) - q - 1), q = ref_logps - logp
  *   (ref_logps NULL: no KL term, kl_coef must be 0); old_logps, advantages, ref_logps fp32 [rows], not looked at in masked rows.  Weights: cu_seqlens NULL
@@ -522,7 +522,7 @@ int ie_logprob_fwd(const void* logits, int dtype, int64_t ld, const int64_t* lab
                    int64_t ignore_index, double inv_temperature, void* stream);
 int ie_logprob_bwd(const void* logits, int dtype, int64_t ld, void* dlogits, int64_t ldd, const int64_t* labels, const float* lse, const float* coef,
                    const float* dloss, float dloss_mul, int64_t rows, int64_t vocab, int64_t ignore_index, double inv_temperature, void* stream);
-int64_t ie_preference_loss_workspace(int64_t pairs);
+int64_t ie_preference_loss_workspace(int64_t rows, int64_t pairs);
 int ie_preference_loss_fwd(const void* logits, int dtype, int64_t ld, const int64_t* labels, const int32_t* cu_seqlens, const float* ref_logps, int kind,
                            double beta, double label_smoothing, double margin, int average, float* loss, float* rewards, float* seq_logps, float* logp,
                            float* lse, float* coef, void* workspace, int64_t rows, int64_t vocab, int64_t pairs, int64_t ignore_index,

@@ -151,7 +151,7 @@ SIGNATURES = {
     "ie_flash_attn_bwd_workspace": (I64, [I64, I, I, I]),
     "ie_logprob_fwd": (I, [P, I, I64, P, P, P, I64, I64, I64, Dbl, P]),
     "ie_logprob_bwd": (I, [P, I, I64, P, I64, P, P, P, P, F, I64, I64, I64, Dbl, P]),
-    "ie_preference_loss_workspace": (I64, [I64]),
+    "ie_preference_loss_workspace": (I64, [I64, I64]),
     "ie_preference_loss_fwd": (I, [P, I, I64, P, P, P, I, Dbl, Dbl, Dbl, I, P, P, P, P, P, P, P, I64, I64, I64, I64, Dbl, P]),
     "ie_policy_loss_workspace": (I64, [I64, I64]),
     "ie_policy_loss": (I, [P, I, I64, P, I64, P, P, P, P, P, I64, F, F, F, P, F, P, P, P, P, P, I64, I64, I64, Dbl, P]),

@@ -68,48 +68,66 @@ template <bool S> __device__ __forceinline__ void stv(void* p, const u32x4& v) {
 }
 
 // Sums of exponentials.  With k = log2(e) / tau:  exp((x - m) / tau) = 2^(x k - r), r = fl(m k): one fma and one exponential an element, m the largest logit so far; what
-// rounding m k loses is the same factor in every term and is taken out of the logarithm at the end (it cancels in p).  The form fails where x k leaves fp32 -- rows in
-// which no logit is above -1e30, such as a vocabulary masked as a whole by the type's lowest value, or whose largest is +inf: those are done over as 2^((x - m) k) (F = false).
+// rounding m k loses is the same factor in every term and goes out again when a thread's sum joins the others'.  The form fails where x k leaves fp32 -- rows in which no
+// logit is above -1e30, such as a vocabulary masked as a whole by the type's lowest value, or whose largest is +inf: those are done over as 2^((x - m) k) (F = false).
 // A maximum that cannot serve counts as none: reference 0, and every term it would belong to is 0 beside any other logit.  NaN and +inf make the sum NaN.
 constexpr float kRange = 1e30f;
 __device__ __forceinline__ float ref(float m, float k) { return m * k >= -kRange ? m * k : 0.f; }
 __device__ __forceinline__ bool in_range(float m, float k) { return fabsf(m * k) <= kRange; }
 template <bool F> __device__ __forceinline__ float term(float x, float k, float r) { return exp2_(F ? __builtin_fmaf(x, k, -r) : (x - r) * k); }
-// sum s of terms that belong to reference r, brought to reference to >= r
-__device__ __forceinline__ float bring(float s, float r, float to) { return s == 0.f ? 0.f : s * exp2_(r - to); }
+
+// log2(e) / tau lies between two fp32 numbers, log2(e) itself 1.3e-8 off the nearer: the same way in every term of every row, which the 500 log-probabilities of a sequence
+// add up to 6e-5.  So the share of threads that its place between them says takes the upper one (a second fma an element would take the error out too: + 4 to 7 %).
+struct Scale {
+    double inv_tau;
+    float lo, hi;
+    unsigned cut;   // of 2^32
+    explicit Scale(double it) : inv_tau(it) {
+        const double e = it * kLog2e;
+        const float f = (float)e;
+        lo = (double)f <= e ? f : nextafterf(f, 0.f);
+        hi = nextafterf(lo, INFINITY);
+        cut = (unsigned)(4294967295.0 * ((e - (double)lo) / ((double)hi - (double)lo)));
+    }
+    __device__ __forceinline__ float mine() const { return threadIdx.x * 0x9e3779b1u < cut ? hi : lo; }   // (multiples of the golden ratio: evenly spread over any threads)
+};
 
 struct RowStat {
-    float m, r, s;   // r: reference of s, m k (fast) or m itself
+    float m, s;   // s = sum exp((x - m) / tau)
     bool fast;
-    // log sum exp((x - m) / tau): the exponent of s apart, so that only the logarithm of a number next to 1 is rounded to 32 bits
-    __device__ __forceinline__ double log_sum(float k) const {
+    // the exponent of s apart, so that only the logarithm of a number next to 1 is rounded to 32 bits
+    __device__ __forceinline__ double log_sum() const {
         int e;
         float f = frexpf(s, &e);
         if (!(f > 0.f) || f == INFINITY) return (double)logf(s);
         if (f < 0.70710678f) { f *= 2.f; --e; }
-        return (double)e * kLn2 + (double)logf(f) - (fast ? ((double)m * (double)k - (double)r) * kLn2 : 0.0);
+        return (double)e * kLn2 + (double)logf(f);
     }
-    __device__ __forceinline__ double lse(double inv_tau, float k) const { return (double)m * inv_tau + log_sum(k); }
-    __device__ __forceinline__ double logp(float x, double inv_tau, float k) const { return ((double)x - (double)m) * inv_tau - log_sum(k); }
+    __device__ __forceinline__ double lse(double inv_tau) const { return (double)m * inv_tau + log_sum(); }
+    __device__ __forceinline__ double logp(float x, double inv_tau) const { return ((double)x - (double)m) * inv_tau - log_sum(); }
 };
 
-// (m, s) of every thread, s at reference ref(m), -> of the workgroup; every thread returns the same.  sh: 2 NT / 64 floats.
+// 2^(r - m k), m the row's maximum, r the reference of a thread's terms: their factor to exp((x - m) / tau)
+__device__ __forceinline__ float to_max(float r, float m, float k) { return exp2_(__builtin_fmaf(-m, k, r)); }
+
+// (m, s) of every thread, s at reference ref(m, k) -> of the workgroup; every thread returns the same.  sh: 2 NT / 64 floats.
 template <int NT>
-__device__ __forceinline__ RowStat join_stats(float m, float s, float k, float* sh) {
+__device__ __forceinline__ RowStat join_stats(float m, float s, float k, float lo, float* sh) {
     constexpr int NW = NT / 64;
     const float wm = wave_max(m);
-    s = wave_sum(bring(s, ref(m, k), ref(wm, k)));
-    if (NW == 1) return {wm, ref(wm, k), s, in_range(wm, k)};
+    s = wave_sum(s == 0.f ? 0.f : s * to_max(ref(m, k), wm, k));
+    if (NW == 1) return {wm, s, in_range(wm, lo)};
     if ((threadIdx.x & 63) == 0) { sh[threadIdx.x >> 6] = wm; sh[NW + (threadIdx.x >> 6)] = s; }
     __syncthreads();
     m = sh[threadIdx.x & (NW - 1)];
+    s = sh[NW + (threadIdx.x & (NW - 1))];
     float b = m;
 #pragma unroll
     for (int o = NW / 2; o > 0; o >>= 1) b = fmaxf(b, __shfl_xor(b, o, 64));
-    s = bring(sh[NW + (threadIdx.x & (NW - 1))], ref(m, k), ref(b, k));
+    s = s == 0.f ? 0.f : s * exp2_((m - b) * lo);
 #pragma unroll
     for (int o = NW / 2; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
-    return {b, ref(b, k), s, in_range(b, k)};
+    return {b, s, in_range(b, lo)};
 }
 
 template <int N>
@@ -117,17 +135,22 @@ __device__ __forceinline__ void add_values(const float* v, float k, float& m, fl
     float c = v[0];
 #pragma unroll
     for (int e = 1; e < N; ++e) c = fmaxf(c, v[e]);
-    if (c > m) { s = bring(s, ref(m, k), ref(c, k)); m = c; }
+    if (c > m) {
+        s = s == 0.f ? 0.f : s * exp2_(ref(m, k) - ref(c, k));
+        m = c;
+    }
     const float r = ref(m, k);
 #pragma unroll
     for (int e = 0; e < N; ++e) s += term<true>(v[e], k, r);
 }
 
+__device__ __forceinline__ float max_ref(float m) { return m == -INFINITY ? 0.f : m; }
+
 // The row whose maximum m is out of the fast form's range, again.  sh as in join_stats, free to be written after the barrier at its start.
 template <bool BF, int NT>
 __device__ __noinline__ RowStat row_stat_again(const typename Elem<BF>::T* x, int vocab, float m, float k, float* sh) {
     constexpr int NW = NT / 64;
-    const float r = m == -INFINITY ? 0.f : m;
+    const float r = max_ref(m);
     float s = 0.f;
     for (int i = threadIdx.x; i < vocab; i += NT) s += term<false>(Elem<BF>::get(x + i), k, r);
     s = wave_sum(s);
@@ -136,13 +159,14 @@ __device__ __noinline__ RowStat row_stat_again(const typename Elem<BF>::T* x, in
     __syncthreads();
     s = 0.f;
     for (int w = 0; w < NW; ++w) s += sh[w];
-    return {m, r, s, false};
+    return {m, s, false};
 }
 
 // One pass over the row, U 16-byte loads a thread in flight.
 template <bool BF, int NT, int U, bool S>
-__device__ __forceinline__ RowStat row_stat(const typename Elem<BF>::T* x, int vocab, float k, float* sh) {
+__device__ __forceinline__ RowStat row_stat(const typename Elem<BF>::T* x, int vocab, const Scale& sc, float* sh) {
     constexpr int N = Elem<BF>::N;
+    const float k = sc.mine();
     float m = -INFINITY, s = 0.f;
     const int nv = vocab / N;
     int i = threadIdx.x;
@@ -173,8 +197,8 @@ __device__ __forceinline__ RowStat row_stat(const typename Elem<BF>::T* x, int v
         const float v = Elem<BF>::get(x + nv * N + threadIdx.x);
         add_values<1>(&v, k, m, s);
     }
-    const RowStat st = join_stats<NT>(m, s, k, sh);
-    return st.fast ? st : row_stat_again<BF, NT>(x, vocab, st.m, k, sh);
+    const RowStat st = join_stats<NT>(m, s, k, sc.lo, sh);
+    return st.fast ? st : row_stat_again<BF, NT>(x, vocab, st.m, sc.lo, sh);
 }
 
 __device__ __forceinline__ bool row_label(const int64_t* labels, int64_t row, int64_t ignore_index, int vocab, int& lab) {
@@ -244,25 +268,31 @@ __device__ __forceinline__ void row_zero(typename Elem<BF>::T* d, int vocab) {
 }
 
 // ------------------------------------------------------------------------------------------ log-probabilities
-// coef (may be null) is cleared: the loss kernels behind this one set it for the rows of their sequences only.
+// coef (may be null) is cleared: the loss kernels behind this one set it for the rows of their sequences only; low comes with it, what logp loses in 32 bits, for sums of
+// many.
 template <bool BF, int NT, bool S>
 __global__ __launch_bounds__(NT) void logprob_fwd_k(const void* __restrict__ logits, int64_t ld, const int64_t* __restrict__ labels, float* __restrict__ logp,
-                                                    float* __restrict__ lse, float* __restrict__ coef, int vocab, int64_t ignore_index, double inv_tau, int64_t row0) {
+                                                    float* __restrict__ lse, float* __restrict__ coef, float* __restrict__ low, int vocab, int64_t ignore_index, Scale sc,
+                                                    int64_t row0) {
     __shared__ float sh[NT / 32];
     const int64_t row = row0 + blockIdx.x;
     int lab;
     if (!row_label(labels, row, ignore_index, vocab, lab)) {
-        if (threadIdx.x == 0) { logp[row] = 0.f; lse[row] = 0.f; if (coef) coef[row] = 0.f; }
+        if (threadIdx.x == 0) {
+            logp[row] = 0.f;
+            lse[row] = 0.f;
+            if (coef) { coef[row] = 0.f; low[row] = 0.f; }
+        }
         return;
     }
     const typename Elem<BF>::T* x = (const typename Elem<BF>::T*)logits + row * ld;
     const float xl = Elem<BF>::get(x + lab);
-    const float k = (float)(inv_tau * kLog2e);
-    const RowStat st = row_stat<BF, NT, 4, S>(x, vocab, k, sh);
+    const RowStat st = row_stat<BF, NT, 4, S>(x, vocab, sc, sh);
     if (threadIdx.x == 0) {
-        lse[row] = (float)st.lse(inv_tau, k);
-        logp[row] = (float)st.logp(xl, inv_tau, k);
-        if (coef) coef[row] = 0.f;
+        const double lp = st.logp(xl, sc.inv_tau);
+        lse[row] = (float)st.lse(sc.inv_tau);
+        logp[row] = (float)lp;
+        if (coef) { coef[row] = 0.f; low[row] = (float)(lp - (double)(float)lp); }
     }
 }
 
@@ -271,7 +301,7 @@ __global__ __launch_bounds__(NT) void logprob_fwd_k(const void* __restrict__ log
 template <bool BF, int NT, bool S>
 __global__ __launch_bounds__(NT) void logprob_bwd_k(const void* logits, int64_t ld, void* dlogits, int64_t ldd, const int64_t* __restrict__ labels,
                                                     const float* __restrict__ lse, const float* __restrict__ coef, const float* __restrict__ dloss, float dloss_mul,
-                                                    int vocab, int64_t ignore_index, double inv_tau, double log2e, int64_t row0, int parts) {
+                                                    int vocab, int64_t ignore_index, Scale sc, double log2e, int64_t row0, int parts) {
     typedef typename Elem<BF>::T T;
     constexpr int N = Elem<BF>::N;
     __shared__ float sh[NT / 32];
@@ -281,7 +311,7 @@ __global__ __launch_bounds__(NT) void logprob_bwd_k(const void* logits, int64_t 
     const T* x = (const T*)logits + row * ld;
     int lab;
     const bool valid = row_label(labels, row, ignore_index, vocab, lab);
-    float g = valid ? coef[row] * dloss_mul * (float)inv_tau : 0.f;
+    float g = valid ? coef[row] * dloss_mul * (float)sc.inv_tau : 0.f;
     if (dloss) g *= dloss[0];
     const int e = part == parts - 1 ? nv * N + (int)threadIdx.x : vocab;   // the row's last elements, fewer than a vector
     if (!valid || g == 0.f) {
@@ -290,15 +320,15 @@ __global__ __launch_bounds__(NT) void logprob_bwd_k(const void* logits, int64_t 
         return;
     }
     // p = 2^(x k - l), l = lse log2(e): what rounding l to 32 bits loses goes into the factor
-    const float k = (float)(inv_tau * kLog2e);
+    const float k = sc.lo;
     const double l = (double)lse[row] * log2e;
     const float r = (float)l;
     if (!(fabsf(r) <= kRange)) {   // out of the fast form's range, where the log-sum-exp cannot hold the sum beside the maximum: one workgroup for the whole row
         if (part != 0) return;
         const float xl = Elem<BF>::get(x + lab);
-        const RowStat st = row_stat<BF, NT, 4, S>(x, vocab, k, sh);
+        const RowStat st = row_stat<BF, NT, 4, S>(x, vocab, sc, sh);
         __syncthreads();           // the row is read before any store may replace it
-        row_grad_again<BF, NT>(x, d, vocab, k, st.r, g, g / st.s, lab, xl);
+        row_grad_again<BF, NT>(x, d, vocab, k, max_ref(st.m), g, g / st.s, lab, xl);
         return;
     }
     const float g_p = g * exp2_((float)((double)r - l));
@@ -362,7 +392,7 @@ __device__ __forceinline__ double pair_loss(const PrefArgs& a, double h, double&
 }
 
 struct PrefRows {
-    const float* logp;
+    const float *logp, *low;   // log-probability = logp + low
     const int64_t* labels;
     const int32_t* cu;
     const float* ref;
@@ -385,7 +415,7 @@ __device__ __forceinline__ void pref_sums(const PrefRows& r, int64_t s, int sub,
     int n = 0;
 #pragma unroll 4
     for (int64_t t = begin + sub * 64 + (threadIdx.x & 63); t < end; t += G * 64) {
-        l += (double)r.logp[t];
+        l += (double)r.logp[t] + (double)r.low[t];
         n += pref_label(r, t) ? 1 : 0;
     }
     sum = wave_sum_d(l);
@@ -621,7 +651,7 @@ __global__ __launch_bounds__(1024) void policy_small_k(PolicyArgs a, const float
 // registers, as exponentials in 32 bits; what a longer row has beyond them (REST) is read again, from the caches.
 template <bool BF, int NT, int NV, bool REST, bool S>
 __global__ __launch_bounds__(NT) void policy_fused_k(PolicyArgs a, const void* logits, int64_t ld, void* dlogits, int64_t ldd, float* __restrict__ logp_out,
-                                                     float* __restrict__ lse_out, const float* __restrict__ dloss, float dloss_mul, double inv_tau, int64_t row0) {
+                                                     float* __restrict__ lse_out, const float* __restrict__ dloss, float dloss_mul, Scale sc, int64_t row0) {
     typedef typename Elem<BF>::T T;
     constexpr int N = Elem<BF>::N;
     __shared__ float sh[NT / 32];
@@ -638,7 +668,7 @@ __global__ __launch_bounds__(NT) void policy_fused_k(PolicyArgs a, const void* l
     }
     // everything the coefficient will need is asked for before the row's own loads, which it would otherwise wait behind
     const PolicyRow in = policy_row(a, row);
-    const float scale = dloss_mul * dloss[0] * (float)inv_tau;
+    const float scale = dloss_mul * dloss[0] * (float)sc.inv_tau;
     int64_t seq, begin, end;
     const bool inside = policy_range(a, row, seq, begin, end);
     int n = 0;
@@ -655,7 +685,7 @@ __global__ __launch_bounds__(NT) void policy_fused_k(PolicyArgs a, const void* l
     }
     const T* x = (const T*)logits + row * ld;
     const float xl = Elem<BF>::get(x + lab);
-    const float k = (float)(inv_tau * kLog2e);
+    const float k = sc.mine();
     const int nv = vocab / N;
     float ex[NV * N], ex_last = -INFINITY;
     {
@@ -686,9 +716,9 @@ __global__ __launch_bounds__(NT) void policy_fused_k(PolicyArgs a, const void* l
     s += ex_last = term<true>(ex_last, k, own);
 #pragma unroll
     for (int q = 0; q < NV * N; ++q) s += ex[q] = term<true>(ex[q], k, own);
-    RowStat st = join_stats<NT>(m, s, k, sh);
-    own = m * k >= -kRange ? exp2_(own - st.r) : 0.f;   // now: the factor of the thread's terms
-    if (!st.fast) st = row_stat_again<BF, NT>(x, vocab, st.m, k, sh);
+    RowStat st = join_stats<NT>(m, s, k, sc.lo, sh);
+    own = m * k >= -kRange ? to_max(own, st.m, k) : 0.f;   // now: the factor of the thread's terms
+    if (!st.fast) st = row_stat_again<BF, NT>(x, vocab, st.m, sc.lo, sh);
     if (!a.counts) {
 #pragma unroll
         for (int q = 0; q < kCountRows; ++q) n += __popcll(__ballot(live >> q & 1u));
@@ -699,9 +729,9 @@ __global__ __launch_bounds__(NT) void policy_fused_k(PolicyArgs a, const void* l
         for (int w = 0; w < NT / 64; ++w) n += counted[w];
     }
     if (threadIdx.x == 0) {
-        const double logp = st.logp(xl, inv_tau, k);
+        const double logp = st.logp(xl, sc.inv_tau);
         logp_out[row] = (float)logp;
-        lse_out[row] = (float)st.lse(inv_tau, k);
+        lse_out[row] = (float)st.lse(sc.inv_tau);
         coef_sh = a.coef[row] = policy_term(a, in, logp, policy_weight(a, inside, n), a.terms[row]);
     }
     __syncthreads();
@@ -709,7 +739,7 @@ __global__ __launch_bounds__(NT) void policy_fused_k(PolicyArgs a, const void* l
     if (g == 0.f) { row_zero<BF, NT, S>(d, vocab); return; }
     const float g_p = g / st.s;
     if (!st.fast) {
-        row_grad_again<BF, NT>(x, d, vocab, k, st.r, g, g_p, lab, xl);
+        row_grad_again<BF, NT>(x, d, vocab, sc.lo, max_ref(st.m), g, g_p, lab, xl);
         return;
     }
     const float f = -g_p * own;
@@ -721,10 +751,11 @@ __global__ __launch_bounds__(NT) void policy_fused_k(PolicyArgs a, const void* l
         for (int q = 0; q < N; ++q) e[q] = f * ex[j * N + q];
         if (i < nv) stv<S>(d + (int64_t)i * N, Elem<BF>::pack(e));
     }
+    const float r = st.m * sc.lo, g_r = g_p * to_max(r, st.m, sc.lo);   // for what is raised again
     if (REST)
-        for (int i = NV * NT + threadIdx.x; i < nv; i += NT) stv<S>(d + (int64_t)i * N, grad_vector<BF, true>(ldv<false>(x + (int64_t)i * N), k, st.r, g_p));
+        for (int i = NV * NT + threadIdx.x; i < nv; i += NT) stv<S>(d + (int64_t)i * N, grad_vector<BF, true>(ldv<false>(x + (int64_t)i * N), sc.lo, r, g_r));
     if (nv * N + (int)threadIdx.x < vocab) Elem<BF>::put(d + nv * N + threadIdx.x, f * ex_last);
-    if (owns<BF, NT>(lab, vocab)) Elem<BF>::put(d + lab, g - g_p * term<true>(xl, k, st.r));
+    if (owns<BF, NT>(lab, vocab)) Elem<BF>::put(d + lab, g - g_r * term<true>(xl, sc.lo, r));
 }
 
 // stats = {loss, surrogate, KL, clipped share}
@@ -779,19 +810,20 @@ struct Launch {
 // Threads a row.  Forward, 8000 x 4000 bf16: 64 threads 17.3 us, 256 17.8, 512 31; 2000 x 32 000 bf16: 256 22.0, 512 22.6, 1024 24.0; 3001 x 32 003 fp32: 256 54, 512 49,
 // 1024 48; 16 384 x 92 544 bf16: 256 266, 512 259, 1024 260; with fewer rows than two a CU the widest workgroup is the shortest wait.
 template <bool BF, bool S>
-void launch_fwd(const Launch& l, int nv, const void* logits, int64_t ld, const int64_t* labels, float* logp, float* lse, float* coef, int vocab, int64_t ignore_index, double inv_tau) {
-    if (nv <= 256) l.go<64>(logprob_fwd_k<BF, 64, S>, logits, ld, labels, logp, lse, coef, vocab, ignore_index, inv_tau);
-    else if (nv <= 4096 && (l.rows >= 512 || nv <= 1024)) l.go<256>(logprob_fwd_k<BF, 256, S>, logits, ld, labels, logp, lse, coef, vocab, ignore_index, inv_tau);
-    else l.go<1024>(logprob_fwd_k<BF, 1024, S>, logits, ld, labels, logp, lse, coef, vocab, ignore_index, inv_tau);
+void launch_fwd(const Launch& l, int nv, const void* logits, int64_t ld, const int64_t* labels, float* logp, float* lse, float* coef, float* low, int vocab, int64_t ignore_index,
+                const Scale& sc) {
+    if (nv <= 256) l.go<64>(logprob_fwd_k<BF, 64, S>, logits, ld, labels, logp, lse, coef, low, vocab, ignore_index, sc);
+    else if (nv <= 4096 && (l.rows >= 512 || nv <= 1024)) l.go<256>(logprob_fwd_k<BF, 256, S>, logits, ld, labels, logp, lse, coef, low, vocab, ignore_index, sc);
+    else l.go<1024>(logprob_fwd_k<BF, 1024, S>, logits, ld, labels, logp, lse, coef, low, vocab, ignore_index, sc);
 }
 
 template <bool BF, bool S>
 void launch_bwd(const Launch& l, int nv, const void* logits, int64_t ld, void* dlogits, int64_t ldd, const int64_t* labels, const float* lse, const float* coef, const float* dloss,
-                float dloss_mul, int vocab, int64_t ignore_index, double inv_tau) {
-    const double log2e = (double)(float)(inv_tau * kLog2e) / inv_tau;   // lse in units of the kernel's x k
+                float dloss_mul, int vocab, int64_t ignore_index, const Scale& sc) {
+    const double log2e = (double)sc.lo / sc.inv_tau;   // lse in units of the kernel's x k
     const int small = (nv + 63) / 64, parts = (nv + 255) / 256;
-    if (nv <= 128) l.parts<64>(logprob_bwd_k<BF, 64, S>, std::max(small, 1), logits, ld, dlogits, ldd, labels, lse, coef, dloss, dloss_mul, vocab, ignore_index, inv_tau, log2e);
-    else l.parts<256>(logprob_bwd_k<BF, 256, S>, parts, logits, ld, dlogits, ldd, labels, lse, coef, dloss, dloss_mul, vocab, ignore_index, inv_tau, log2e);
+    if (nv <= 128) l.parts<64>(logprob_bwd_k<BF, 64, S>, std::max(small, 1), logits, ld, dlogits, ldd, labels, lse, coef, dloss, dloss_mul, vocab, ignore_index, sc, log2e);
+    else l.parts<256>(logprob_bwd_k<BF, 256, S>, parts, logits, ld, dlogits, ldd, labels, lse, coef, dloss, dloss_mul, vocab, ignore_index, sc, log2e);
 }
 
 // Threads and vectors a thread of the fused kernel, so that the row fills most of them and two workgroups share a CU while they can.  bf16, rows x vocabulary:
@@ -801,15 +833,15 @@ inline int fused_threads(int nv) { return nv <= 256 ? 64 : nv <= 2048 ? 256 : nv
 
 template <bool BF, bool S>
 void launch_fused(const Launch& l, int nv, const PolicyArgs& a, const void* logits, int64_t ld, void* dlogits, int64_t ldd, float* logp, float* lse, const float* dloss, float dloss_mul,
-                  double inv_tau) {
-    if (nv <= 128) l.go<64>(policy_fused_k<BF, 64, 2, false, S>, a, logits, ld, dlogits, ldd, logp, lse, dloss, dloss_mul, inv_tau);
-    else if (nv <= 256) l.go<64>(policy_fused_k<BF, 64, 4, false, S>, a, logits, ld, dlogits, ldd, logp, lse, dloss, dloss_mul, inv_tau);
-    else if (nv <= 1024) l.go<256>(policy_fused_k<BF, 256, 4, false, S>, a, logits, ld, dlogits, ldd, logp, lse, dloss, dloss_mul, inv_tau);
-    else if (nv <= 2048) l.go<256>(policy_fused_k<BF, 256, 8, false, S>, a, logits, ld, dlogits, ldd, logp, lse, dloss, dloss_mul, inv_tau);
-    else if (nv <= 4096) l.go<512>(policy_fused_k<BF, 512, 8, false, S>, a, logits, ld, dlogits, ldd, logp, lse, dloss, dloss_mul, inv_tau);
-    else if (nv <= 6656) l.go<512>(policy_fused_k<BF, 512, 10, true, S>, a, logits, ld, dlogits, ldd, logp, lse, dloss, dloss_mul, inv_tau);
-    else if (nv <= 8192) l.go<1024>(policy_fused_k<BF, 1024, 8, false, S>, a, logits, ld, dlogits, ldd, logp, lse, dloss, dloss_mul, inv_tau);
-    else l.go<1024>(policy_fused_k<BF, 1024, BF ? 10 : 16, true, S>, a, logits, ld, dlogits, ldd, logp, lse, dloss, dloss_mul, inv_tau);
+                  const Scale& sc) {
+    if (nv <= 128) l.go<64>(policy_fused_k<BF, 64, 2, false, S>, a, logits, ld, dlogits, ldd, logp, lse, dloss, dloss_mul, sc);
+    else if (nv <= 256) l.go<64>(policy_fused_k<BF, 64, 4, false, S>, a, logits, ld, dlogits, ldd, logp, lse, dloss, dloss_mul, sc);
+    else if (nv <= 1024) l.go<256>(policy_fused_k<BF, 256, 4, false, S>, a, logits, ld, dlogits, ldd, logp, lse, dloss, dloss_mul, sc);
+    else if (nv <= 2048) l.go<256>(policy_fused_k<BF, 256, 8, false, S>, a, logits, ld, dlogits, ldd, logp, lse, dloss, dloss_mul, sc);
+    else if (nv <= 4096) l.go<512>(policy_fused_k<BF, 512, 8, false, S>, a, logits, ld, dlogits, ldd, logp, lse, dloss, dloss_mul, sc);
+    else if (nv <= 6656) l.go<512>(policy_fused_k<BF, 512, 10, true, S>, a, logits, ld, dlogits, ldd, logp, lse, dloss, dloss_mul, sc);
+    else if (nv <= 8192) l.go<1024>(policy_fused_k<BF, 1024, 8, false, S>, a, logits, ld, dlogits, ldd, logp, lse, dloss, dloss_mul, sc);
+    else l.go<1024>(policy_fused_k<BF, 1024, BF ? 10 : 16, true, S>, a, logits, ld, dlogits, ldd, logp, lse, dloss, dloss_mul, sc);
 }
 
 // fn<type, stream>(args...)
@@ -834,7 +866,7 @@ extern "C" int ie_logprob_fwd(const void* logits, int dtype, int64_t ld, const i
     IE_CHECK_ARG(logits && labels && logp && lse, "ie_logprob_fwd: null pointer");
     IE_CHECK_LOGITS("ie_logprob_fwd");
     if (rows == 0) return IE_OK;
-    IE_ROWS(launch_fwd, logits, ld, labels, logp, lse, (float*)nullptr, (int)vocab, ignore_index, inv_temperature);
+    IE_ROWS(launch_fwd, logits, ld, labels, logp, lse, (float*)nullptr, (float*)nullptr, (int)vocab, ignore_index, Scale(inv_temperature));
     return ie_launch_status("ie_logprob_fwd launch");
 }
 
@@ -844,11 +876,12 @@ extern "C" int ie_logprob_bwd(const void* logits, int dtype, int64_t ld, void* d
     IE_CHECK_LOGITS("ie_logprob_bwd");
     IE_CHECK_ARG(ldd >= vocab && overlap_ok(logits, ld, dlogits, ldd, rows, vocab, dtype), "ie_logprob_bwd: dlogits must be the logits themselves or lie apart from them");
     if (rows == 0) return IE_OK;
-    IE_ROWS(launch_bwd, logits, ld, dlogits, ldd, labels, lse, coef, dloss, dloss_mul, (int)vocab, ignore_index, inv_temperature);
+    IE_ROWS(launch_bwd, logits, ld, dlogits, ldd, labels, lse, coef, dloss, dloss_mul, (int)vocab, ignore_index, Scale(inv_temperature));
     return ie_launch_status("ie_logprob_bwd launch");
 }
 
-extern "C" int64_t ie_preference_loss_workspace(int64_t pairs) { return pairs > 0 ? pairs * 8 : 0; }
+// the pairs' losses in 64 bits, then what the log-probabilities lose in 32
+extern "C" int64_t ie_preference_loss_workspace(int64_t rows, int64_t pairs) { return rows >= 0 && pairs > 0 ? pairs * 8 + rows * 4 : 0; }
 
 extern "C" int ie_preference_loss_fwd(const void* logits, int dtype, int64_t ld, const int64_t* labels, const int32_t* cu_seqlens, const float* ref_logps, int kind,
                                       double beta, double label_smoothing, double margin, int average, float* loss, float* rewards, float* seq_logps, float* logp,
@@ -863,10 +896,11 @@ extern "C" int ie_preference_loss_fwd(const void* logits, int dtype, int64_t ld,
                  "ie_preference_loss_fwd: label smoothing lies in [0, 0.5] and belongs to the sigmoid form");
     IE_CHECK_ARG(margin >= -1e30 && margin <= 1e30 && (kind != IE_PREF_IPO || margin == 0.0), "ie_preference_loss_fwd: the squared form takes no margin");
     hipStream_t st = (hipStream_t)stream;
-    if (rows > 0) IE_ROWS(launch_fwd, logits, ld, labels, logp, lse, coef, (int)vocab, ignore_index, inv_temperature);
-    const PrefArgs a = {kind, average, beta, label_smoothing, margin};
-    const PrefRows r = {logp, labels, cu_seqlens, ref_logps, rows, pairs, ignore_index, (int)vocab, rewards, seq_logps, coef};
     double* losses = (double*)workspace;
+    float* low = (float*)(losses + pairs);
+    if (rows > 0) IE_ROWS(launch_fwd, logits, ld, labels, logp, lse, coef, low, (int)vocab, ignore_index, Scale(inv_temperature));
+    const PrefArgs a = {kind, average, beta, label_smoothing, margin};
+    const PrefRows r = {logp, low, labels, cu_seqlens, ref_logps, rows, pairs, ignore_index, (int)vocab, rewards, seq_logps, coef};
     if (pairs <= kOnePairs && rows <= kOneRows) {
         if (pairs == 1) hipLaunchKernelGGL((preference_pairs_k<8, false>), dim3(1), dim3(1024), 0, st, r, a, loss, losses);
         else if (pairs == 2) hipLaunchKernelGGL((preference_pairs_k<4, false>), dim3(1), dim3(1024), 0, st, r, a, loss, losses);
@@ -903,16 +937,16 @@ extern "C" int ie_policy_loss(const void* logits, int dtype, int64_t ld, void* d
     a.coef = coef; a.rows = rows; a.seqs = seqs; a.ignore_index = ignore_index; a.vocab = (int)vocab;
     a.low = clip_low; a.high = clip_high; a.kl_coef = kl_coef;
     if (!dlogits && rows <= kSmallRows && seqs <= kSmallSeqs) {
-        if (rows > 0) IE_ROWS(launch_fwd, logits, ld, labels, logp, lse, (float*)nullptr, (int)vocab, ignore_index, inv_temperature);
+        if (rows > 0) IE_ROWS(launch_fwd, logits, ld, labels, logp, lse, (float*)nullptr, (float*)nullptr, (int)vocab, ignore_index, Scale(inv_temperature));
         hipLaunchKernelGGL(policy_small_k, dim3(1), dim3(1024), 0, st, a, (const float*)logp, stats);
         return ie_launch_status("ie_policy_loss launch");
     }
     if (dlogits && rows <= (int64_t)kCountRows * fused_threads(vectors(vocab, dtype))) a.counts = nullptr;
     else hipLaunchKernelGGL(policy_counts_k, dim3((unsigned)(cu_seqlens ? seqs : 1)), dim3(1024), 0, st, a, counts);
     if (rows > 0 && dlogits) {
-        IE_ROWS(launch_fused, a, logits, ld, dlogits, ldd, logp, lse, dloss, dloss_mul, inv_temperature);
+        IE_ROWS(launch_fused, a, logits, ld, dlogits, ldd, logp, lse, dloss, dloss_mul, Scale(inv_temperature));
     } else if (rows > 0) {
-        IE_ROWS(launch_fwd, logits, ld, labels, logp, lse, (float*)nullptr, (int)vocab, ignore_index, inv_temperature);
+        IE_ROWS(launch_fwd, logits, ld, labels, logp, lse, (float*)nullptr, (float*)nullptr, (int)vocab, ignore_index, Scale(inv_temperature));
         hipLaunchKernelGGL(policy_terms_k, dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, a, (const float*)logp);
     }
     hipLaunchKernelGGL(policy_stats_k, dim3(1), dim3(1024), 0, st, (const float4*)workspace, rows, kl_coef, stats);

@@ -304,7 +304,7 @@ class PreferenceLoss:
     def __init__(self, rows, small, seqs):
         self._rows, self._small, self._seqs = rows, small, seqs
 
-    loss = property(lambda self: self._small[2 * self._seqs:2 * self._seqs + 1])
+    loss = property(lambda self: self._small[2 * self._seqs:])
     rewards = property(lambda self: self._small[:self._seqs].view(-1, 2))
     seq_logps = property(lambda self: self._small[self._seqs:2 * self._seqs])
     logp = property(lambda self: self._rows[0])
@@ -452,12 +452,12 @@ def preference_loss_fwd(logits, labels, cu_seqlens, ref_logps=None, beta=0.1, ki
     stream = _raw_stream(_on_current_device(logits, labels, cu_seqlens, ref_logps))
     L = _L()
     per_row = torch.empty((3, rows), dtype=torch.float32, device=logits.device)
-    ws = L.ie_preference_loss_workspace(seqs // 2) // 4
-    small = per_row.new_empty(2 * seqs + 2 + ws)   # rewards, seq_logps, loss, then (8-byte values: 2 seqs + 2 is even) the workspace
+    small = per_row.new_empty(2 * seqs + 1)   # rewards, seq_logps, loss
+    ws = per_row.new_empty(L.ie_preference_loss_workspace(rows, seqs // 2) // 4)
     p, q = _ptr(per_row), small.data_ptr()
     step = 4 * rows
     check(L.ie_preference_loss_fwd(_ptr(logits), dt, ld, _ptr(labels), cu_seqlens.data_ptr(), _ptr(ref_logps), _PREFERENCE_KINDS[kind], beta, label_smoothing, margin,
-                                   bool(average), q + 8 * seqs, q, q + 4 * seqs, p, p + step, p + 2 * step, q + 8 * seqs + 8, rows, V, seqs // 2, ignore_index, inv,
+                                   bool(average), q + 8 * seqs, q, q + 4 * seqs, p, p + step, p + 2 * step, ws.data_ptr(), rows, V, seqs // 2, ignore_index, inv,
                                    stream), "ie_preference_loss_fwd")
     return PreferenceLoss(per_row, small, seqs)
 

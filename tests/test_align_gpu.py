@@ -152,7 +152,9 @@ def test_infinite_and_nan_logits_in_live_rows(dev, dtype):
 
 
 def pref_ref(logp, labels, cu, ref, beta, kind, eps, margin, average):
-    """64-bit loss, rewards, sums and coefficients from given log-probabilities"""
+    """64-bit loss, rewards, sums and coefficients from given log-probabilities, and what the loss, the rewards and the coefficients may be off: the kernel sums its
+    log-probabilities before they are rounded to 32 bits, u |lp| each and all of one sign, so that a sum may be off by u |sum|; the loss by its slope times that, a
+    coefficient by the loss's second derivative times that -- at most beta^2 / 4, 0 and 2 of the three forms"""
     lp, lab = logp.cpu().double(), labels.cpu()
     S = len(cu) - 1
     sums = torch.zeros(S, dtype=torch.float64)
@@ -177,7 +179,14 @@ def pref_ref(logp, labels, cu, ref, beta, kind, eps, margin, average):
     for s in range(S):
         if live[s]:
             coef[live[s]] = h0.grad[s] / (len(live[s]) if average else 1)
-    return loss.detach(), beta * h0.detach(), sums, coef
+    off = U * sums.abs()
+    bend = {"sigmoid": beta ** 2 / 4, "hinge": 0.0, "ipo": 2.0}[kind] / (S // 2) * (off[0::2] + off[1::2])
+    coef_off = torch.zeros_like(coef)
+    for s in range(S):
+        coef_off[live[s]] = bend[s // 2] / (max(1, len(live[s])) if average else 1)
+    tol = ((h0.grad.abs() * off).sum() + 2 * U * loss.detach().abs() + 1e-12, beta * off + 2 * U * (beta * h0.detach()).abs() + 1e-12,
+           coef_off + 2 * U * coef.abs() + 2.0 ** -50)   # (the slope of a saturated sigmoid is a difference of 64-bit values: absolute 2^-50)
+    return loss.detach(), beta * h0.detach(), sums, coef, tol
 
 
 PREF = [dict(kind="sigmoid"), dict(kind="sigmoid", label_smoothing=0.2, margin=0.4), dict(kind="sigmoid", average=True, beta=2.0, margin=0.5), dict(kind="hinge", margin=0.3),
@@ -193,19 +202,18 @@ def test_preference_loss(dev, cu, opt, dtype):
     S = len(cu) - 1
     base = K().token_logprobs(x, y)[0]
     g = torch.Generator().manual_seed(3)
-    _, _, sums, _ = pref_ref(base, y, cu, None, 1.0, "sigmoid", 0, 0, opt.get("average", False))
+    _, _, sums, _, _ = pref_ref(base, y, cu, None, 1.0, "sigmoid", 0, 0, opt.get("average", False))
     for with_ref in (True, False):
         ref = (sums + torch.randn(S, generator=g).double() / opt.get("beta", 0.1)).float().to(dev) if with_ref else None
         r = K().preference_loss_fwd(x, y, torch.tensor(cu, dtype=torch.int32, device=dev), ref, **opt)
         assert torch.equal(r.logp, base)
         args = (opt.get("beta", 0.1), opt["kind"], opt.get("label_smoothing", 0.0), opt.get("margin", 0.0), opt.get("average", False))
-        loss, rewards, sums_, coef = pref_ref(r.logp, y, cu, ref, *args)
+        loss, rewards, sums_, coef, tol = pref_ref(r.logp, y, cu, ref, *args)
         assert r.loss.shape == (1,) and r.rewards.shape == (S // 2, 2)
-        check(r.loss, loss.reshape(1), 2 * U * loss.abs() + 1e-12, "loss")
+        check(r.loss, loss.reshape(1), tol[0], "loss")
         check(r.seq_logps, sums_, 2 * U * sums_.abs(), "seq_logps")
-        check(r.rewards, rewards.reshape(-1, 2), 2 * U * rewards.abs().reshape(-1, 2) + 1e-12, "rewards")
-        # (the slope of a saturated sigmoid is a difference of 64-bit values: absolute 2^-50)
-        check(r.coef, coef, 2 * U * coef.abs() + 2.0 ** -50, "coef")
+        check(r.rewards, rewards.reshape(-1, 2), tol[1].reshape(-1, 2), "rewards")
+        check(r.coef, coef, tol[2], "coef")
         dloss = torch.full((1,), 64.0, device=dev)
         d = K().preference_loss_bwd(x, y, r, dloss, 0.5, dlogits=torch.empty_like(x))
         check_dlogits(d, x, y, r.coef.double() * 32.0, "dlogits")
@@ -218,10 +226,22 @@ def test_preference_loss_of_many_pairs_and_of_long_ones(dev):
         cu = [0] + sorted(torch.randint(0, rows + 1, (S - 1,), generator=g).tolist()) + [rows]
         ref = torch.randn(S, generator=g).to(dev)
         r = K().preference_loss_fwd(x, y, torch.tensor(cu, dtype=torch.int32, device=dev), ref, average=True)
-        loss, rewards, sums, coef = pref_ref(r.logp, y, cu, ref, 0.1, "sigmoid", 0.0, 0.0, True)
-        check(r.loss, loss.reshape(1), 2 * U, "loss")
+        loss, rewards, sums, coef, tol = pref_ref(r.logp, y, cu, ref, 0.1, "sigmoid", 0.0, 0.0, True)
+        check(r.loss, loss.reshape(1), tol[0], "loss")
         check(r.seq_logps, sums, 2 * U * sums.abs(), "seq_logps")
-        check(r.coef, coef, 2 * U * coef.abs() + 2.0 ** -50, "coef")
+        check(r.coef, coef, tol[2], "coef")
+
+
+def test_sums_of_a_long_sequence_keep_their_digits(dev):
+    """3000 log-probabilities a sequence against 64 bits: their errors are rounding errors of 32-bit sums, independent from row to row (u sqrt(V / 256 + 64) each, five
+    times the deviation of the sum allowed), and no common bias is left (the rounding of log2(e) alone would be 1.3e-8 of every row's mean distance from its maximum)."""
+    rows, V = 6000, 3001
+    x, y = make(dev, rows, V, torch.float32, 12, mask=0.0)
+    r = K().preference_loss_fwd(x, y, torch.tensor([0, 3000, 6000], dtype=torch.int32, device=dev))
+    lp = ref_logp(x, y)[0]
+    for s in range(2):
+        want = float(lp[3000 * s:3000 * s + 3000].sum())
+        assert abs(float(r.seq_logps[s]) - want) <= U * abs(want) + 5 * U * math.sqrt(3000 * (V / 256 + 64)), (float(r.seq_logps[s]), want)
 
 
 def test_broken_offsets_stay_inside_the_rows(dev):

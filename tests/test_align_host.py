@@ -217,7 +217,7 @@ def test_gradient_list_entries_refuse_bad_calls(lib):
 
 
 def test_workspace_sizes(lib):
-    assert lib.ie_preference_loss_workspace(3) == 24
+    assert lib.ie_preference_loss_workspace(10, 3) == 64
     assert lib.ie_policy_loss_workspace(10, 0) == 41 * 4 and lib.ie_policy_loss_workspace(10, 4) == 44 * 4
     # one launch at least, and one more for every full set of tensors
     assert lib.ie_grad_norm_workspace(0) > 0 and lib.ie_grad_norm_workspace(1000) > lib.ie_grad_norm_workspace(1)
