@@ -173,7 +173,7 @@ def prepare(case, seed):
         grads = []
         shapes = _shapes(case)
         if case["odd"]:   # views into two flat buffers, each one element behind the last: most of them start at an unaligned address
-            flats = {t: randn(sum(n + 1 for n, d in shapes if d == t) + 1, dtype=t).mul_(0.01) for t in {d for _, d in shapes}}
+            flats = {t: randn(sum(n + 1 for n, d in shapes if d == t) + 1, dtype=t).mul_(0.01) for t in _DTYPES.values()}
             at = dict.fromkeys(flats, 1)
             for n, t in shapes:
                 grads.append(flats[t][at[t]:at[t] + n])
@@ -226,17 +226,16 @@ def prepare(case, seed):
 
 # ------------------------------------------------------------------------------------------------ plain forms
 def _plain_softmax(logits, labels, temperature):
-    """Log-probabilities and log-sum-exps, valid rows, exponentials and their sums.  Long sums and their logarithms are in 64 bits: a log-probability is the small difference of
-    two numbers near 20, and a sequence adds up hundreds of them."""
+    """Log-probabilities and log-sum-exps in 64 bits from 32-bit sums (a log-probability is the small difference of two numbers near 20, and a sequence adds up hundreds of
+    them), valid rows, exponentials and their sums."""
     z = logits.float() / temperature
     m = z.amax(1, keepdim=True)
     e = torch.exp(z - m)
-    s = e.sum(1, keepdim=True, dtype=torch.float64)
-    log_s = torch.log(s)[:, 0]
+    s = e.sum(1, keepdim=True)
+    log_s = torch.log(s.double())[:, 0]
     valid = labels >= 0
-    logp = (z.gather(1, labels.clamp(min=0)[:, None]) - m)[:, 0].double() - log_s
-    zero = torch.zeros_like(log_s)
-    return torch.where(valid, logp, zero), torch.where(valid, m[:, 0].double() + log_s, zero), valid, e, s.float()
+    logp = (z.gather(1, labels.clamp(min=0)[:, None]) - m)[:, 0] - log_s
+    return torch.where(valid, logp, 0.0), torch.where(valid, m[:, 0] + log_s, 0.0), valid, e, s
 
 
 def _plain_dlogits(logits, labels, valid, e, s, dlogp, temperature):
