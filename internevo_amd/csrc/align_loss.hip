@@ -80,13 +80,14 @@ template <bool F> __device__ __forceinline__ float term(float x, float k, float 
 // add up to 6e-5.  So the share of threads that its place between them says takes the upper one (a second fma an element would take the error out too: + 4 to 7 %).
 struct Scale {
     double inv_tau;
-    float lo, hi;
-    unsigned cut;   // of 2^32
+    float lo, hi, rest;   // rest: log2(e) / tau - lo
+    unsigned cut;         // of 2^32
     explicit Scale(double it) : inv_tau(it) {
         const double e = it * kLog2e;
         const float f = (float)e;
         lo = (double)f <= e ? f : nextafterf(f, 0.f);
         hi = nextafterf(lo, INFINITY);
+        rest = (float)(e - (double)lo);
         cut = (unsigned)(4294967295.0 * ((e - (double)lo) / ((double)hi - (double)lo)));
     }
     __device__ __forceinline__ float mine() const { return threadIdx.x * 0x9e3779b1u < cut ? hi : lo; }   // (multiples of the golden ratio: evenly spread over any threads)
@@ -95,28 +96,27 @@ struct Scale {
 struct RowStat {
     float m, s;   // s = sum exp((x - m) / tau)
     bool fast;
-    // the exponent of s apart, so that only the logarithm of a number next to 1 is rounded to 32 bits
-    __device__ __forceinline__ double log_sum() const {
-        int e;
-        float f = frexpf(s, &e);
-        if (!(f > 0.f) || f == INFINITY) return (double)logf(s);
-        if (f < 0.70710678f) { f *= 2.f; --e; }
-        return (double)e * kLn2 + (double)logf(f);
-    }
+    __device__ __forceinline__ double log_sum() const { return log((double)s); }
     __device__ __forceinline__ double lse(double inv_tau) const { return (double)m * inv_tau + log_sum(); }
     __device__ __forceinline__ double logp(float x, double inv_tau) const { return ((double)x - (double)m) * inv_tau - log_sum(); }
 };
 
-// 2^(r - m k), m the row's maximum, r the reference of a thread's terms: their factor to exp((x - m) / tau)
-__device__ __forceinline__ float to_max(float r, float m, float k) { return exp2_(__builtin_fmaf(-m, k, r)); }
+// exp(d / tau) 2^lost: whole sums are multiplied by it, so the exponent is taken apart into a whole number and a remainder and nothing of it is rounded away
+__device__ __forceinline__ float shift(float d, float lost, const Scale& sc) {
+    const float n = rintf(d * sc.lo);
+    if (!(n >= -160.f)) return exp2_(n);   // (0, or NaN)
+    return ldexpf(exp2_(__builtin_fmaf(d, sc.lo, -n) + __builtin_fmaf(d, sc.rest, lost)), (int)n);
+}
+// factor that brings a thread's terms 2^(x k - ref(m, k)) to exp((x - to) / tau)
+__device__ __forceinline__ float to_max(float m, float k, float to, const Scale& sc) { return shift(m - to, __builtin_fmaf(-m, k, ref(m, k)), sc); }
 
 // (m, s) of every thread, s at reference ref(m, k) -> of the workgroup; every thread returns the same.  sh: 2 NT / 64 floats.
 template <int NT>
-__device__ __forceinline__ RowStat join_stats(float m, float s, float k, float lo, float* sh) {
+__device__ __forceinline__ RowStat join_stats(float m, float s, float k, const Scale& sc, float* sh) {
     constexpr int NW = NT / 64;
     const float wm = wave_max(m);
-    s = wave_sum(s == 0.f ? 0.f : s * to_max(ref(m, k), wm, k));
-    if (NW == 1) return {wm, s, in_range(wm, lo)};
+    s = wave_sum(s == 0.f ? 0.f : s * to_max(m, k, wm, sc));
+    if (NW == 1) return {wm, s, in_range(wm, sc.lo)};
     if ((threadIdx.x & 63) == 0) { sh[threadIdx.x >> 6] = wm; sh[NW + (threadIdx.x >> 6)] = s; }
     __syncthreads();
     m = sh[threadIdx.x & (NW - 1)];
@@ -124,10 +124,24 @@ __device__ __forceinline__ RowStat join_stats(float m, float s, float k, float l
     float b = m;
 #pragma unroll
     for (int o = NW / 2; o > 0; o >>= 1) b = fmaxf(b, __shfl_xor(b, o, 64));
-    s = s == 0.f ? 0.f : s * exp2_((m - b) * lo);
+    s = s == 0.f ? 0.f : s * shift(m - b, 0.f, sc);
 #pragma unroll
     for (int o = NW / 2; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
-    return {b, s, in_range(b, lo)};
+    return {b, s, in_range(b, sc.lo)};
+}
+
+// Sum of N values (a power of two) as a tree: a term next to 1 -- the label's, in a trained model -- meets log2 N roundings, where one sum from left to right would
+// round the others away one by one
+template <int N>
+__device__ __forceinline__ float tree_sum(const float* v) {
+    float t[N];
+#pragma unroll
+    for (int e = 0; e < N; ++e) t[e] = v[e];
+#pragma unroll
+    for (int w = N / 2; w > 0; w >>= 1)
+#pragma unroll
+        for (int e = 0; e < w; ++e) t[e] += t[e + w];
+    return t[0];
 }
 
 template <int N>
@@ -140,8 +154,10 @@ __device__ __forceinline__ void add_values(const float* v, float k, float& m, fl
         m = c;
     }
     const float r = ref(m, k);
+    float t[N];
 #pragma unroll
-    for (int e = 0; e < N; ++e) s += term<true>(v[e], k, r);
+    for (int e = 0; e < N; ++e) t[e] = term<true>(v[e], k, r);
+    s += tree_sum<N>(t);
 }
 
 __device__ __forceinline__ float max_ref(float m) { return m == -INFINITY ? 0.f : m; }
@@ -197,7 +213,7 @@ __device__ __forceinline__ RowStat row_stat(const typename Elem<BF>::T* x, int v
         const float v = Elem<BF>::get(x + nv * N + threadIdx.x);
         add_values<1>(&v, k, m, s);
     }
-    const RowStat st = join_stats<NT>(m, s, k, sc.lo, sh);
+    const RowStat st = join_stats<NT>(m, s, k, sc, sh);
     return st.fast ? st : row_stat_again<BF, NT>(x, vocab, st.m, sc.lo, sh);
 }
 
@@ -515,17 +531,18 @@ struct PolicyArgs {
 };
 
 // tokens with a label, per sequence (cu) or in all (cu null, one workgroup)
-__global__ __launch_bounds__(1024) void policy_counts_k(PolicyArgs a, int32_t* __restrict__ counts) {
-    __shared__ double scratch[16];
+template <int NT>
+__global__ __launch_bounds__(NT) void policy_counts_k(PolicyArgs a, int32_t* __restrict__ counts) {
+    __shared__ double scratch[NT / 64];
     int64_t begin = 0, end = a.rows;
     if (a.cu) seq_range(a.cu, blockIdx.x, a.rows, begin, end);
     int n = 0;
 #pragma unroll 8
-    for (int64_t t = begin + threadIdx.x; t < end; t += 1024) {
+    for (int64_t t = begin + threadIdx.x; t < end; t += NT) {
         int lab;
         n += row_label(a.labels, t, a.ignore_index, a.vocab, lab) ? 1 : 0;
     }
-    const double total = block_sum_d<16>((double)n, scratch);
+    const double total = block_sum_d<NT / 64>((double)n, scratch);
     if (threadIdx.x == 0) counts[blockIdx.x] = (int32_t)total;
 }
 
@@ -533,10 +550,13 @@ __global__ __launch_bounds__(1024) void policy_counts_k(PolicyArgs a, int32_t* _
 __device__ __forceinline__ bool policy_range(const PolicyArgs& a, int64_t t, int64_t& s, int64_t& begin, int64_t& end) {
     s = 0; begin = 0; end = a.rows;
     if (!a.cu) return true;
-    for (int64_t i = 0; i < a.seqs; i += 64) {   // how many of cu[1..S] are <= t
-        const int64_t j = i + (threadIdx.x & 63);
-        s += __popcll(__ballot(j < a.seqs && (int64_t)a.cu[min(j, a.seqs - 1) + 1] <= t));
+    int64_t left = a.seqs;   // how many of cu[1..S] are <= t: halved down to a wave's width, then one look
+    while (left > 64) {
+        const int64_t half = left >> 1;
+        if ((int64_t)a.cu[s + half] <= t) { s += half; left -= half; } else left = half;
     }
+    const int64_t lane = threadIdx.x & 63;
+    s += __popcll(__ballot(lane < left && (int64_t)a.cu[s + min(lane, left - 1) + 1] <= t));
     if (s >= a.seqs) return false;
     seq_range(a.cu, s, a.rows, begin, end);
     return t >= begin && t < end;
@@ -650,7 +670,7 @@ __global__ __launch_bounds__(1024) void policy_small_k(PolicyArgs a, const float
 // Forward and backward of one row: its coefficient needs nothing but the row itself, so the logits are read once.  NV vectors a thread wait in
 // registers, as exponentials in 32 bits; what a longer row has beyond them (REST) is read again, from the caches.
 template <bool BF, int NT, int NV, bool REST, bool S>
-__global__ __launch_bounds__(NT) void policy_fused_k(PolicyArgs a, const void* logits, int64_t ld, void* dlogits, int64_t ldd, float* __restrict__ logp_out,
+__global__ __launch_bounds__(NT, NT >= 512 ? 4 : 1) void policy_fused_k(PolicyArgs a, const void* logits, int64_t ld, void* dlogits, int64_t ldd, float* __restrict__ logp_out,
                                                      float* __restrict__ lse_out, const float* __restrict__ dloss, float dloss_mul, Scale sc, int64_t row0) {
     typedef typename Elem<BF>::T T;
     constexpr int N = Elem<BF>::N;
@@ -715,9 +735,13 @@ __global__ __launch_bounds__(NT) void policy_fused_k(PolicyArgs a, const void* l
     float own = ref(m, k);   // reference of the thread's terms
     s += ex_last = term<true>(ex_last, k, own);
 #pragma unroll
-    for (int q = 0; q < NV * N; ++q) s += ex[q] = term<true>(ex[q], k, own);
-    RowStat st = join_stats<NT>(m, s, k, sc.lo, sh);
-    own = m * k >= -kRange ? to_max(own, st.m, k) : 0.f;   // now: the factor of the thread's terms
+    for (int j = 0; j < NV; ++j) {
+#pragma unroll
+        for (int q = 0; q < N; ++q) ex[j * N + q] = term<true>(ex[j * N + q], k, own);
+        s += tree_sum<N>(ex + j * N);
+    }
+    RowStat st = join_stats<NT>(m, s, k, sc, sh);
+    own = m * k >= -kRange ? to_max(m, k, st.m, sc) : 0.f;   // now: the factor of the thread's terms
     if (!st.fast) st = row_stat_again<BF, NT>(x, vocab, st.m, sc.lo, sh);
     if (!a.counts) {
 #pragma unroll
@@ -751,7 +775,7 @@ __global__ __launch_bounds__(NT) void policy_fused_k(PolicyArgs a, const void* l
         for (int q = 0; q < N; ++q) e[q] = f * ex[j * N + q];
         if (i < nv) stv<S>(d + (int64_t)i * N, Elem<BF>::pack(e));
     }
-    const float r = st.m * sc.lo, g_r = g_p * to_max(r, st.m, sc.lo);   // for what is raised again
+    const float r = st.m * sc.lo, g_r = g_p * exp2_(__builtin_fmaf(-st.m, sc.lo, r));   // for what is raised again
     if (REST)
         for (int i = NV * NT + threadIdx.x; i < nv; i += NT) stv<S>(d + (int64_t)i * N, grad_vector<BF, true>(ldv<false>(x + (int64_t)i * N), sc.lo, r, g_r));
     if (nv * N + (int)threadIdx.x < vocab) Elem<BF>::put(d + nv * N + threadIdx.x, f * ex_last);
@@ -888,6 +912,7 @@ extern "C" int ie_preference_loss_fwd(const void* logits, int dtype, int64_t ld,
                                       float* lse, float* coef, void* workspace, int64_t rows, int64_t vocab, int64_t pairs, int64_t ignore_index, double inv_temperature,
                                       void* stream) {
     IE_CHECK_ARG(logits && labels && cu_seqlens && loss && rewards && seq_logps && logp && lse && coef && workspace, "ie_preference_loss_fwd: null pointer");
+    IE_CHECK_ARG(((uintptr_t)workspace & 7) == 0, "ie_preference_loss_fwd: the workspace must be 8-byte aligned");
     IE_CHECK_LOGITS("ie_preference_loss_fwd");
     IE_CHECK_ARG(pairs > 0 && pairs <= kMaxSeqs / 2, "ie_preference_loss_fwd: at least one pair");
     IE_CHECK_ARG(kind == IE_PREF_SIGMOID || kind == IE_PREF_HINGE || kind == IE_PREF_IPO, "ie_preference_loss_fwd: unknown kind");
@@ -942,7 +967,8 @@ extern "C" int ie_policy_loss(const void* logits, int dtype, int64_t ld, void* d
         return ie_launch_status("ie_policy_loss launch");
     }
     if (dlogits && rows <= (int64_t)kCountRows * fused_threads(vectors(vocab, dtype))) a.counts = nullptr;
-    else hipLaunchKernelGGL(policy_counts_k, dim3((unsigned)(cu_seqlens ? seqs : 1)), dim3(1024), 0, st, a, counts);
+    else if (cu_seqlens) hipLaunchKernelGGL((policy_counts_k<256>), dim3((unsigned)seqs), dim3(256), 0, st, a, counts);
+    else hipLaunchKernelGGL((policy_counts_k<1024>), dim3(1), dim3(1024), 0, st, a, counts);
     if (rows > 0 && dlogits) {
         IE_ROWS(launch_fused, a, logits, ld, dlogits, ldd, logp, lse, dloss, dloss_mul, Scale(inv_temperature));
     } else if (rows > 0) {

@@ -373,6 +373,7 @@ extern "C" int64_t ie_grad_norm_workspace(int64_t n) { return n < 0 ? 0 : (n / k
 
 extern "C" int ie_grad_norm(const void* const* ptrs, const int64_t* numels, const int* dtypes, int64_t n, void* workspace, float* norm, void* stream) {
     IE_CHECK_ARG(workspace && norm, "ie_grad_norm: null pointer");
+    IE_CHECK_ARG(((uintptr_t)workspace & 7) == 0, "ie_grad_norm: the workspace must be 8-byte aligned");
     Lists l = {ptrs, numels, dtypes, nullptr, nullptr, n, 0, 0, 0, false};
     const int rc = check_list("ie_grad_norm: bad tensor list", l);
     if (rc != IE_OK) return rc;
@@ -384,6 +385,7 @@ extern "C" int ie_grad_norm(const void* const* ptrs, const int64_t* numels, cons
 extern "C" int ie_grad_clip(const void* const* ptrs, const int64_t* numels, const int* dtypes, void* const* outs, const int* out_dtypes, int64_t n, double max_norm,
                             void* workspace, float* norm, void* stream) {
     IE_CHECK_ARG(workspace && norm, "ie_grad_clip: null pointer");
+    IE_CHECK_ARG(((uintptr_t)workspace & 7) == 0, "ie_grad_clip: the workspace must be 8-byte aligned");
     IE_CHECK_ARG(max_norm >= 0.0, "ie_grad_clip: max_norm must not be negative");
     Lists l = {ptrs, numels, dtypes, outs, out_dtypes, n, 0, 0, 0, false};
     int rc = check_list("ie_grad_clip: bad tensor list", l);

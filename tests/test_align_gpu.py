@@ -304,8 +304,9 @@ def policy_ref(logp, labels, old, adv, ref, low, high, kl_coef, cu):
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=["bf16", "fp32"])
 @pytest.mark.parametrize("kl", [None, 0.0, 0.1])
-@pytest.mark.parametrize("rows, V, cu", [(1, 33, None), (37, 517, None), (1500, 65, None), (40, 1031, [0, 13, 13, 40]), (25, 32003, [2, 9, 20]), (3000, 40, list(range(0, 2701, 27)))],
-                         ids=["one-row", "tokens", "many", "sequences", "rows-outside", "100-sequences"])
+@pytest.mark.parametrize("rows, V, cu", [(1, 33, None), (37, 517, None), (1500, 65, None), (40, 1031, [0, 13, 13, 40]), (25, 32003, [2, 9, 20]), (3000, 40, list(range(0, 2701, 27))),
+                                          (5000, 9, [3 + 3 * i - (i % 2) for i in range(1600)])],
+                         ids=["one-row", "tokens", "many", "sequences", "rows-outside", "100-sequences", "1599-sequences"])
 def test_policy_loss(dev, rows, V, cu, kl, dtype):
     low, high, tau = 0.2, 0.28, 0.8
     x, y = make(dev, rows, V, dtype, rows + V, pad=3, mask=0.3 if rows > 1 else 0.0)
@@ -489,6 +490,11 @@ def test_grad_norm_and_clip(dev, kind):
             check(o, r, (torch.finfo(o.dtype).eps / 2 + 4 * U) * r.abs() + 1e-38, "in place")
             if f == 1.0:
                 assert torch.equal(t, o)
+
+
+def test_lists_without_an_element(dev):
+    ts = [torch.empty(0, device=dev), torch.empty(0, dtype=torch.bfloat16, device=dev)]
+    assert float(K().grad_norm(ts)) == 0.0 and float(K().clip_grad_norm_(ts, 1.0)) == 0.0
 
 
 def test_clip_leaves_neighbours_alone(dev):

@@ -158,6 +158,7 @@ def test_c_entries_refuse_bad_calls(lib):
         return lib.ie_preference_loss_fwd(f, 0, 8, f, f, None, kind, beta, smooth, margin, 0, f, f, f, f, f, f, ws, 4, 8, pairs, -100, 1.0, None)
 
     _refused(lib, pref(ws=None), "null")
+    _refused(lib, pref(ws=ctypes.c_void_p(4100)), "aligned")
     _refused(lib, pref(pairs=0), "pair")
     _refused(lib, pref(kind=3), "kind")
     for b in (0.0, -0.1, float("nan"), float("inf")):
@@ -192,6 +193,7 @@ def test_gradient_list_entries_refuse_bad_calls(lib):
         return lib.ie_grad_norm(*_arrays(ptrs, numels, dtypes), len(ptrs) if n is None else n, ws, FAKE, None)
 
     _refused(lib, norm([4096], [8], [0], ws=None), "null")
+    _refused(lib, norm([4096], [8], [0], ws=ctypes.c_void_p(4100)), "aligned")
     _refused(lib, norm([4096], [-1], [0]), "list")
     _refused(lib, norm([None], [8], [0]), "list")
     _refused(lib, norm([4096], [8], [2]), "list")
