@@ -1,5 +1,9 @@
+import fcntl
+import multiprocessing.process
 import os
 import sys
+import tempfile
+import time
 
 import pytest
 
@@ -70,6 +74,65 @@ def pytest_configure(config):
     config.addinivalue_line("markers", "gpu: needs a real MI355X (run with -m gpu on the GPU box)")
     config.addinivalue_line("markers", "ranks(n): GPUs a multi-rank test needs for its RCCL (nccl backend) variant")
     config.addinivalue_line("markers", "extended: a parametrisation whose layout another default test covers; run with IE_TEST_FULL=1")
+
+
+# A device takes few processes at once (16 where this suite was measured), and which tests of several ranks meet on the four workers changes with the number of
+# tests.  So the ranks of all workers together draw from one pool of _SLOTS places: 4 workers + 10 ranks, whatever the order.  A test says how many it
+# needs by the processes that it has made when it starts the first of them, and gives them back at its end; a place is a locked file, so that a dead worker's are free.
+_SLOTS = 10
+_SUBPROCESS_RANKS = 3   # a test that starts the benchmark program: two ranks and their parent
+_made, _held = [], []
+_process_init, _process_start = multiprocessing.process.BaseProcess.__init__, multiprocessing.process.BaseProcess.start
+
+
+def _take_slots(n):
+    folder = os.path.join(tempfile.gettempdir(), "ie_ranks_%s_%d" % (os.environ.get("PYTEST_XDIST_TESTRUNUID", "serial%d" % os.getpid()), os.getuid()))
+    os.makedirs(folder, exist_ok=True)
+    with open(os.path.join(folder, "turn"), "w") as turn:
+        fcntl.flock(turn, fcntl.LOCK_EX)   # (one worker waits for places at a time: two that hold a part each cannot wait for each other)
+        free = list(range(_SLOTS))
+        while len(_held) < min(n, _SLOTS):
+            for i in list(free):
+                if len(_held) == min(n, _SLOTS):
+                    break
+                f = open(os.path.join(folder, str(i)), "w")
+                try:
+                    fcntl.flock(f, fcntl.LOCK_EX | fcntl.LOCK_NB)
+                except OSError:
+                    f.close()
+                    continue
+                _held.append(f)
+                free.remove(i)
+            if len(_held) < min(n, _SLOTS):
+                time.sleep(0.05)
+
+
+@pytest.hookimpl(hookwrapper=True)
+def pytest_runtest_call(item):
+    if item.get_closest_marker("gpu") is None:
+        yield
+        return
+
+    def init(self, *args, **kw):
+        _process_init(self, *args, **kw)
+        _made.append(self)
+
+    def start(self):
+        if not _held:
+            _take_slots(len(_made))
+        _process_start(self)
+
+    multiprocessing.process.BaseProcess.__init__, multiprocessing.process.BaseProcess.start = init, start
+    try:
+        if "subprocess" in getattr(getattr(item.obj, "__code__", None), "co_names", ()) + getattr(getattr(item.obj, "__code__", None), "co_varnames", ()):
+            _take_slots(_SUBPROCESS_RANKS)
+        yield
+    finally:
+        multiprocessing.process.BaseProcess.__init__, multiprocessing.process.BaseProcess.start = _process_init, _process_start
+        for f in _held:
+            f.close()
+        _held.clear()
+        _made.clear()
 
 
 @pytest.fixture(scope="session")
