@@ -274,6 +274,21 @@ __device__ __noinline__ void row_grad_again(const typename Elem<BF>::T* x, typen
     row_grad<BF, NT, 1, false, false>(x, d, vocab, k, r, g, g_p, lab, xl);
 }
 
+// A log-sum-exp in 32 bits is off by up to half its last place, and so is every probability formed with it: 2^-18 of it below 128, 2^-14 below 2048.  Beyond
+// what the gradient's type shows of that (small temperatures, logits far from zero) a row's sums are formed again.
+template <bool BF> constexpr float kFar = BF ? 2048.f * 1.4426950f : 128.f * 1.4426950f;   // (in units of log 2)
+
+template <bool BF, int NT, bool S>
+__device__ __forceinline__ void row_grad_far(const typename Elem<BF>::T* x, typename Elem<BF>::T* d, int vocab, float g, int lab, const Scale& sc, float* sh) {
+    const float xl = Elem<BF>::get(x + lab);
+    const RowStat st = row_stat<BF, NT, 2, S>(x, vocab, sc, sh);
+    __syncthreads();   // the row is read before any store may replace it
+    const float k = sc.lo, g_p = g / st.s;
+    if (!st.fast) { row_grad_again<BF, NT>(x, d, vocab, k, max_ref(st.m), g, g_p, lab, xl); return; }
+    const float r = st.m * k;
+    row_grad<BF, NT, 2, S, true>(x, d, vocab, k, r, g, g_p * exp2_(__builtin_fmaf(-st.m, k, r)), lab, xl);
+}
+
 template <bool BF, int NT, bool S>
 __device__ __forceinline__ void row_zero(typename Elem<BF>::T* d, int vocab) {
     constexpr int N = Elem<BF>::N;
@@ -339,12 +354,8 @@ __global__ __launch_bounds__(NT) void logprob_bwd_k(const void* logits, int64_t 
     const float k = sc.lo;
     const double l = (double)lse[row] * log2e;
     const float r = (float)l;
-    if (!(fabsf(r) <= kRange)) {   // out of the fast form's range, where the log-sum-exp cannot hold the sum beside the maximum: one workgroup for the whole row
-        if (part != 0) return;
-        const float xl = Elem<BF>::get(x + lab);
-        const RowStat st = row_stat<BF, NT, 4, S>(x, vocab, sc, sh);
-        __syncthreads();           // the row is read before any store may replace it
-        row_grad_again<BF, NT>(x, d, vocab, k, max_ref(st.m), g, g / st.s, lab, xl);
+    if (!(fabsf(r) <= kFar<BF>)) {   // the row's sums again, by one workgroup
+        if (part == 0) row_grad_far<BF, NT, S>(x, d, vocab, g, lab, sc, sh);
         return;
     }
     const float g_p = g * exp2_((float)((double)r - l));
@@ -795,8 +806,8 @@ __global__ __launch_bounds__(1024) void policy_stats_k(const float4* __restrict_
 }
 
 constexpr int64_t kMaxVocab = int64_t(1) << 30;   // in-row indices are 32-bit
-constexpr int64_t kMaxRows = (int64_t(1) << 26) - 1;   // (a launch of a wave a row has fewer than 2^32 threads)
-constexpr int64_t kMaxSeqs = (int64_t(1) << 22) - 1;   // ... of 1024 threads a sequence
+constexpr int64_t kMaxRows = (int64_t(1) << 26) - 4;   // (a launch of a wave a row, four a workgroup, has fewer than 2^32 threads)
+constexpr int64_t kMaxSeqs = (int64_t(1) << 22) - 1;   // ... and one of 1024 threads a pair fewer than half of that
 
 #define IE_CHECK_LOGITS(fn)                                                                                                                              \
     IE_CHECK_ARG(dtype == IE_BF16 || dtype == IE_F32, fn ": bad dtype");                                                                                 \

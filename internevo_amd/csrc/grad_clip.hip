@@ -267,6 +267,8 @@ struct Lists {
     bool stream;   // beyond the 256 MB of the last-level cache: past it
 };
 
+constexpr int64_t kMostBlocks = (int64_t(1) << 22) - 1;   // workgroups of 1024 threads a launch: fewer than 2^32 threads
+
 int check_list(const char* msg, Lists& l) {
     if (l.n < 0 || l.n > (int64_t(1) << 24) || (l.n > 0 && (!l.ptrs || !l.numels || !l.dtypes))) { ie_set_error(msg); return IE_ERR_INVALID; }
     l.elems = l.bytes = 0;
@@ -277,10 +279,12 @@ int check_list(const char* msg, Lists& l) {
         }
         l.elems += l.numels[i];
         l.bytes += l.numels[i] * esize(l.dtypes[i]);
+        if (l.elems > (int64_t(1) << 48)) { ie_set_error(msg); return IE_ERR_INVALID; }
     }
-    // 4096 chunks or more, where the list is long enough for it
+    // 4096 chunks or more, where the list is long enough for it; longer ones where one tensor stands in it so often that a launch could not hold all its tensors' chunks
+    // (the workspace is made for launches of kNormTensors)
     l.shift = kMinShift;
-    while (l.shift < kMaxShift && (l.elems >> l.shift) > 4096) ++l.shift;
+    while ((l.shift < kMaxShift && (l.elems >> l.shift) > 4096) || (l.elems >> l.shift) > kMostBlocks - kNormTensors) ++l.shift;
     l.stream = l.bytes > (int64_t(256) << 20);
     return IE_OK;
 }
@@ -291,26 +295,26 @@ inline int64_t blocks_of(const ClipList& t, const Lists& l, int64_t i) {
     const int64_t steps = l.numels[i] / step_of(in, out) + l.numels[i] % step_of(in, out), per = (int64_t)kClipThreads * t.u * t.rounds;   // (whole steps, then elements)
     return (steps + per - 1) / per;
 }
-inline void longer(NormList& t) { ++t.shift; }
-inline void longer(ClipList& t) { t.rounds *= 2; }
+inline void fit(NormList&, const Lists&, int64_t) {}   // (the whole list's chunks fit one launch)
+inline void fit(ClipList& t, const Lists& l, int64_t i) {
+    while (blocks_of(t, l, i) > kMostBlocks) t.rounds *= 2;
+}
 inline void put_out(NormList&, int, const Lists&, int64_t) {}
 inline void put_out(ClipList& t, int k, const Lists& l, int64_t i) {
     t.out[k] = l.outs ? l.outs[i] : (void*)l.ptrs[i];
     if ((l.outs ? l.out_dtypes[i] : l.dtypes[i]) == IE_BF16) t.len[k] |= kOutBf;
 }
 
-// the next launch's tensors, from i on; returns where the one after it starts.  A launch has fewer than 2^22 workgroups (2^32 threads); a tensor that needs more of them
-// alone gets longer chunks.
+// the next launch's tensors, from i on; returns where the one after it starts.  A tensor that needs more workgroups alone than a launch has gets several rounds each.
 template <int CAP, typename L>
 int64_t fill(L& t, int64_t i, const Lists& l) {
-    constexpr int64_t most = (int64_t(1) << 22) - 1;
     t.n = 0;
     int64_t total = 0;
     for (; i < l.n && t.n < CAP; ++i) {
         if (l.numels[i] == 0) continue;
-        while (t.n == 0 && blocks_of(t, l, i) > most) longer(t);
+        if (t.n == 0) fit(t, l, i);
         const int64_t chunks = blocks_of(t, l, i);
-        if (total + chunks > most) break;
+        if (total + chunks > kMostBlocks) break;
         t.in[t.n] = l.ptrs[i];
         t.len[t.n] = l.numels[i] | (l.dtypes[i] == IE_BF16 ? kBf : 0);
         put_out(t, t.n, l, i);

@@ -151,6 +151,31 @@ def test_infinite_and_nan_logits_in_live_rows(dev, dtype):
     assert bool(d[3].isnan().all()) and bool(d[4].isnan().all())
 
 
+@pytest.mark.parametrize("dtype", DTYPES, ids=["bf16", "fp32"])
+@pytest.mark.parametrize("centre, temperature", [(100.0, 1.0), (-300.0, 1.0), (5000.0, 1.0), (-40000.0, 3.0), (0.0, 0.01), (2.0, 1e-3)])
+def test_gradient_of_rows_far_from_zero(dev, centre, temperature, dtype):
+    """The gradient keeps its digits where the log-sum-exp is large.  A saved log-sum-exp below 128 (fp32 gradients) or 2048 (bf16) is off by 2^-18 or 2^-14 at
+    most; everything else goes with the distance from it, not with its size."""
+    for V in (90, 5003):
+        x, y = make(dev, 9, V, dtype, V, 2, 1, 0.2, scale=3.0 * temperature)
+        x += centre
+        _, lse = K().token_logprobs(x, y, temperature=temperature)
+        c = torch.linspace(0.5, 2.0, 9, device=dev)
+        d = K().token_logprobs_bwd(x, y, lse, c, temperature=temperature, dlogits=torch.full_like(x, 7.0))
+        _, ls, valid, z = ref_logp(x, y, temperature)
+        p = torch.exp(z - ls[:, None])
+        hot = torch.zeros_like(p)
+        hot[torch.arange(9)[valid], y.cpu()[valid]] = 1.0
+        g = (torch.where(valid, c.cpu().double(), torch.zeros(())) / temperature)[:, None]
+        ref = torch.where(g != 0, g * (hot - p), torch.zeros(()))
+        eps = torch.finfo(dtype).eps / 2
+        share = U * (V / 256 + 64 + 8 + 4 * (z - ls[:, None]).abs()) + (2.0 ** -14 if dtype == torch.bfloat16 else 2.0 ** -18)
+        check(d, ref, (eps + 4 * U) * ref.abs() + g.abs() * p * share + 2 * U * g.abs() * hot + 2.0 ** -125 * (1 + g.abs()), f"dlogits, {V} columns")
+        inplace = x.clone()
+        K().token_logprobs_bwd(inplace, y, lse, c, temperature=temperature)
+        assert torch.equal(inplace, d)
+
+
 def pref_ref(logp, labels, cu, ref, beta, kind, eps, margin, average):
     """64-bit loss, rewards, sums and coefficients from given log-probabilities, and what the loss, the rewards and the coefficients may be off: the kernel sums its
     log-probabilities before they are rounded to 32 bits, u |lp| each and all of one sign, so that a sum may be off by u |sum|; the loss by its slope times that, a
@@ -490,6 +515,12 @@ def test_grad_norm_and_clip(dev, kind):
             check(o, r, (torch.finfo(o.dtype).eps / 2 + 4 * U) * r.abs() + 1e-38, "in place")
             if f == 1.0:
                 assert torch.equal(t, o)
+
+
+def test_norm_of_one_tensor_many_times(dev):
+    """more elements in all than one launch's chunks of the usual length hold (the tensors of a real list would not fit the card)"""
+    t = torch.ones(1 << 30, dtype=torch.bfloat16, device=dev)
+    assert float(K().grad_norm([t] * 300)) == pytest.approx(math.sqrt(300 * 2.0 ** 30), rel=2 * U)
 
 
 def test_lists_without_an_element(dev):

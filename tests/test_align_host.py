@@ -147,6 +147,7 @@ def test_c_entries_refuse_bad_calls(lib):
     _refused(lib, lib.ie_logprob_fwd(f, 0, 7, f, f, f, 4, 8, -100, 1.0, None), "shape")
     _refused(lib, lib.ie_logprob_fwd(f, 0, 1 << 40, f, f, f, 4, 1 << 31, -100, 1.0, None), "shape")
     _refused(lib, lib.ie_logprob_fwd(f, 0, 8, f, f, f, 1 << 31, 8, -100, 1.0, None), "shape")
+    _refused(lib, lib.ie_logprob_fwd(f, 0, 8, f, f, f, (1 << 26) - 3, 8, -100, 1.0, None), "shape")   # (one workgroup of four rows more than a launch may have)
     for t in (0.0, -1.0, float("nan"), float("inf")):
         _refused(lib, lib.ie_logprob_fwd(f, 0, 8, f, f, f, 4, 8, -100, t, None), "temperature")
     # a gradient that overlaps the logits without being them
@@ -195,6 +196,7 @@ def test_gradient_list_entries_refuse_bad_calls(lib):
     _refused(lib, norm([4096], [8], [0], ws=None), "null")
     _refused(lib, norm([4096], [8], [0], ws=ctypes.c_void_p(4100)), "aligned")
     _refused(lib, norm([4096], [-1], [0]), "list")
+    _refused(lib, norm([4096] * 1025, [1 << 38] * 1025, [0] * 1025), "list")
     _refused(lib, norm([None], [8], [0]), "list")
     _refused(lib, norm([4096], [8], [2]), "list")
     _refused(lib, norm([4096], [8], [0], n=-1), "list")
