@@ -60,7 +60,7 @@ __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(
 constexpr double kLog2e = 1.44269504088896340736;
 constexpr double kLn2 = 0.693147180559945309417;
 
-// S: past the caches (non-temporal), for logits or gradients larger than the last-level cache
+// S (of loads alone: L): past the caches (non-temporal)
 template <bool S> __device__ __forceinline__ u32x4 ldv(const void* p) { return S ? __builtin_nontemporal_load((const u32x4_any*)p) : *(const u32x4_any*)p; }
 template <bool S> __device__ __forceinline__ void stv(void* p, const u32x4& v) {
     if (S) __builtin_nontemporal_store(v, (u32x4_any*)p);
@@ -242,7 +242,7 @@ __device__ __forceinline__ u32x4 grad_vector(const u32x4& w, float k, float r, f
 
 // d = g 1[j = label] - g_p 2^(x k - r) for the whole row: with the row's reference and sum g_p = g / s, with its log-sum-exp as reference g_p = g.  xl: the label's
 // logit, read before any store (dlogits may be the logits themselves).
-template <bool BF, int NT, int U, bool S, bool F>
+template <bool BF, int NT, int U, bool L, bool S, bool F>
 __device__ __forceinline__ void row_grad(const typename Elem<BF>::T* x, typename Elem<BF>::T* d, int vocab, float k, float r, float g, float g_p, int lab, float xl) {
     constexpr int N = Elem<BF>::N;
     const int nv = vocab / N;
@@ -250,7 +250,7 @@ __device__ __forceinline__ void row_grad(const typename Elem<BF>::T* x, typename
     for (; i + (U - 1) * NT < nv; i += U * NT) {
         u32x4 w[U];
 #pragma unroll
-        for (int u = 0; u < U; ++u) w[u] = ldv<S>(x + (int64_t)(i + u * NT) * N);
+        for (int u = 0; u < U; ++u) w[u] = ldv<L>(x + (int64_t)(i + u * NT) * N);
 #pragma unroll
         for (int u = 0; u < U; ++u) stv<S>(d + (int64_t)(i + u * NT) * N, grad_vector<BF, F>(w[u], k, r, g_p));
     }
@@ -258,7 +258,7 @@ __device__ __forceinline__ void row_grad(const typename Elem<BF>::T* x, typename
         u32x4 w[U];
 #pragma unroll
         for (int u = 0; u < U - 1; ++u)
-            if (i + u * NT < nv) w[u] = ldv<S>(x + (int64_t)(i + u * NT) * N);
+            if (i + u * NT < nv) w[u] = ldv<L>(x + (int64_t)(i + u * NT) * N);
 #pragma unroll
         for (int u = 0; u < U - 1; ++u)
             if (i + u * NT < nv) stv<S>(d + (int64_t)(i + u * NT) * N, grad_vector<BF, F>(w[u], k, r, g_p));
@@ -271,22 +271,22 @@ __device__ __forceinline__ void row_grad(const typename Elem<BF>::T* x, typename
 // the same for a row out of the fast form's range
 template <bool BF, int NT>
 __device__ __noinline__ void row_grad_again(const typename Elem<BF>::T* x, typename Elem<BF>::T* d, int vocab, float k, float r, float g, float g_p, int lab, float xl) {
-    row_grad<BF, NT, 1, false, false>(x, d, vocab, k, r, g, g_p, lab, xl);
+    row_grad<BF, NT, 1, false, false, false>(x, d, vocab, k, r, g, g_p, lab, xl);
 }
 
 // A log-sum-exp in 32 bits is off by up to half its last place, and so is every probability formed with it: 2^-18 of it below 128, 2^-14 below 2048.  Beyond
 // what the gradient's type shows of that (small temperatures, logits far from zero) a row's sums are formed again.
 template <bool BF> constexpr float kFar = BF ? 2048.f * 1.4426950f : 128.f * 1.4426950f;   // (in units of log 2)
 
-template <bool BF, int NT, bool S>
+template <bool BF, int NT, bool L, bool S>
 __device__ __forceinline__ void row_grad_far(const typename Elem<BF>::T* x, typename Elem<BF>::T* d, int vocab, float g, int lab, const Scale& sc, float* sh) {
     const float xl = Elem<BF>::get(x + lab);
-    const RowStat st = row_stat<BF, NT, 2, S>(x, vocab, sc, sh);
+    const RowStat st = row_stat<BF, NT, 2, L>(x, vocab, sc, sh);
     __syncthreads();   // the row is read before any store may replace it
     const float k = sc.lo, g_p = g / st.s;
     if (!st.fast) { row_grad_again<BF, NT>(x, d, vocab, k, max_ref(st.m), g, g_p, lab, xl); return; }
     const float r = st.m * k;
-    row_grad<BF, NT, 2, S, true>(x, d, vocab, k, r, g, g_p * exp2_(__builtin_fmaf(-st.m, k, r)), lab, xl);
+    row_grad<BF, NT, 2, L, S, true>(x, d, vocab, k, r, g, g_p * exp2_(__builtin_fmaf(-st.m, k, r)), lab, xl);
 }
 
 template <bool BF, int NT, bool S>
@@ -328,23 +328,57 @@ __global__ __launch_bounds__(NT) void logprob_fwd_k(const void* __restrict__ log
 }
 
 // `parts` workgroups a row, one vector a thread and no loop: the chip's reads and writes then move through memory as one dense front, which HBM serves at 6.6 TB/s of
-// mixed traffic where workgroups that walk a row each get 5.5.  16 384 x 92 544 bf16, 40 % masked: 785 us (a workgroup a row: 871).
-template <bool BF, int NT, bool S>
-__global__ __launch_bounds__(NT) void logprob_bwd_k(const void* logits, int64_t ld, void* dlogits, int64_t ldd, const int64_t* __restrict__ labels,
-                                                    const float* __restrict__ lse, const float* __restrict__ coef, const float* __restrict__ dloss, float dloss_mul,
-                                                    int vocab, int64_t ignore_index, Scale sc, double log2e, int64_t row0, int parts) {
+// mixed traffic where workgroups that walk a row each get 5.5.  16 384 x 92 544 bf16, 40 % masked: 775 us (a workgroup a row: 871).
+// What a workgroup needs before its first vector is asked for in two rounds, the launch's arguments and then the row's numbers, each as a whole (the compiler would
+// put every scalar load next to its use, six rounds one after the other): with one vector a thread the kernel waits for them longer than it works.
+struct Divisor {   // n / d for any 32-bit n by one product (Granlund and Montgomery, 1994)
+    unsigned d, mul, s1, s2;
+    explicit Divisor(unsigned d_) : d(d_) {
+        unsigned l = 0;
+        while (l < 32 && (uint64_t(1) << l) < d) ++l;
+        mul = (unsigned)(((uint64_t(1) << 32) * ((uint64_t(1) << l) - d)) / d + 1);
+        s1 = l < 1 ? l : 1;
+        s2 = l > 1 ? l - 1 : 0;
+    }
+    __device__ __forceinline__ unsigned of(unsigned n) const {
+        const unsigned t = __umulhi(mul, n);
+        return (t + ((n - t) >> s1)) >> s2;
+    }
+};
+template <typename T> __device__ __forceinline__ T sload(const T* p, int64_t i) {   // a scalar load: p[i] is not written while the kernel runs
+    return ((const __attribute__((address_space(4))) T*)p)[i];
+}
+struct BwdArgs {
+    const void* logits;
+    void* dlogits;
+    int64_t ld, ldd;
+    const int64_t* labels;
+    const float *lse, *coef, *dloss;   // dloss: any readable number if there is none
+    int64_t ignore_index;
+    double log2e;                      // lse in units of the kernel's x k
+    float mul, dloss_or;               // 1 / tau and the caller's factor; dloss counts if dloss_or is 0
+    int vocab;
+};
+
+template <bool BF, int NT, bool L, bool S>
+__global__ __launch_bounds__(NT) void logprob_bwd_k(BwdArgs a, Scale sc, Divisor parts, int64_t row0) {
     typedef typename Elem<BF>::T T;
     constexpr int N = Elem<BF>::N;
     __shared__ float sh[NT / 32];
-    const int64_t row = row0 + blockIdx.x / parts;
-    const int part = blockIdx.x % parts, nv = vocab / N, i = part * NT + threadIdx.x;
-    T* d = (T*)dlogits + row * ldd;
-    const T* x = (const T*)logits + row * ld;
-    int lab;
-    const bool valid = row_label(labels, row, ignore_index, vocab, lab);
-    float g = valid ? coef[row] * dloss_mul * (float)sc.inv_tau : 0.f;
-    if (dloss) g *= dloss[0];
-    const int e = part == parts - 1 ? nv * N + (int)threadIdx.x : vocab;   // the row's last elements, fewer than a vector
+    asm volatile("" :: "s"(a.logits), "s"(a.dlogits), "s"(a.ld), "s"(a.ldd), "s"(a.labels), "s"(a.lse), "s"(a.coef), "s"(a.dloss), "s"(a.ignore_index), "s"(a.log2e),
+                 "s"(a.mul), "s"(a.dloss_or), "s"(a.vocab), "s"(row0), "s"(sc.lo));
+    const int vocab = a.vocab;
+    const unsigned slice = parts.of(blockIdx.x);
+    const int64_t row = row0 + slice;
+    const int64_t label = sload(a.labels, row);
+    const float coef = sload(a.coef, row), lse = sload(a.lse, row), dloss = sload(a.dloss, 0);
+    asm volatile("" :: "s"(label), "s"(coef), "s"(lse), "s"(dloss));
+    const int part = (int)(blockIdx.x - slice * parts.d), nv = vocab / N, i = part * NT + threadIdx.x, lab = (int)label;
+    T* d = (T*)a.dlogits + row * a.ldd;
+    const T* x = (const T*)a.logits + row * a.ld;
+    const bool valid = label != a.ignore_index && label >= 0 && label < vocab;
+    const float g = valid ? coef * a.mul * (a.dloss_or == 0.f ? dloss : a.dloss_or) : 0.f;
+    const int e = part == (int)parts.d - 1 ? nv * N + (int)threadIdx.x : vocab;   // the row's last elements, fewer than a vector
     if (!valid || g == 0.f) {
         if (i < nv) stv<S>(d + (int64_t)i * N, u32x4{0, 0, 0, 0});
         if (e < vocab) Elem<BF>::put(d + e, 0.f);
@@ -352,15 +386,15 @@ __global__ __launch_bounds__(NT) void logprob_bwd_k(const void* logits, int64_t 
     }
     // p = 2^(x k - l), l = lse log2(e): what rounding l to 32 bits loses goes into the factor
     const float k = sc.lo;
-    const double l = (double)lse[row] * log2e;
+    const double l = (double)lse * a.log2e;
     const float r = (float)l;
     if (!(fabsf(r) <= kFar<BF>)) {   // the row's sums again, by one workgroup
-        if (part == 0) row_grad_far<BF, NT, S>(x, d, vocab, g, lab, sc, sh);
+        if (part == 0) row_grad_far<BF, NT, L, S>(x, d, vocab, g, lab, sc, sh);
         return;
     }
     const float g_p = g * exp2_((float)((double)r - l));
     if (i < nv) {
-        const u32x4 w = ldv<S>(x + (int64_t)i * N);
+        const u32x4 w = ldv<L>(x + (int64_t)i * N);
         float v[N];
         Elem<BF>::unpack(w, v);
 #pragma unroll
@@ -822,12 +856,14 @@ bool overlap_ok(const void* x, int64_t ld, const void* d, int64_t ldd, int64_t r
     return xb + ((rows - 1) * ld + vocab) * es <= db || db + ((rows - 1) * ldd + vocab) * es <= xb;
 }
 
-// logits beyond the 256 MB of the last-level cache stream past it
-bool streams(int64_t rows, int64_t vocab, int dtype) { return rows * vocab * (dtype == IE_BF16 ? 2 : 4) > (int64_t(256) << 20); }
+// Past the 256 MB of the last-level cache: loads of logits beyond 192 MB, stores where the call touches more than that in all.  30 % of the rows masked, logits just
+// written, forward and backward, loads and stores cached | loads alone | neither: 92 544 bf16 columns, 128 MB in place 53 us | 56 | 58, into other memory 71 | 57 | 59;
+// 192 MB 79 | 80 | 82 and 87 | 81 | 82; 256 MB 120 | 113 | 103 and 120 | 110 | 106; 768 MB 355 | 340 | 276.
+bool beyond(int64_t rows, int64_t vocab, int dtype, bool twice) { return (rows * vocab * (dtype == IE_BF16 ? 2 : 4) << (twice ? 1 : 0)) > (int64_t(192) << 20); }
 
 inline int vectors(int64_t vocab, int dtype) { return (int)(vocab / (dtype == IE_BF16 ? 8 : 4)); }
 
-// rows in slices, so that no launch has 2^32 threads; the kernel's last arguments are the slice's first row, and the workgroups a row if there are several
+// rows in slices, so that no launch has 2^32 threads; the kernel's last argument is the slice's first row, before it the workgroups a row if there are several
 struct Launch {
     hipStream_t st;
     int64_t rows;
@@ -838,7 +874,7 @@ struct Launch {
     template <int NT, typename F, typename... A> void parts(F f, int parts, A... args) const {
         const int64_t most = ((int64_t(1) << 32) / NT - 1) / parts;
         for (int64_t row0 = 0; row0 < rows; row0 += most)
-            hipLaunchKernelGGL(f, dim3((unsigned)(std::min(most, rows - row0) * parts)), dim3(NT), 0, st, args..., row0, parts);
+            hipLaunchKernelGGL(f, dim3((unsigned)(std::min(most, rows - row0) * parts)), dim3(NT), 0, st, args..., Divisor((unsigned)parts), row0);
     }
 };
 
@@ -852,13 +888,10 @@ void launch_fwd(const Launch& l, int nv, const void* logits, int64_t ld, const i
     else l.go<1024>(logprob_fwd_k<BF, 1024, S>, logits, ld, labels, logp, lse, coef, low, vocab, ignore_index, sc);
 }
 
-template <bool BF, bool S>
-void launch_bwd(const Launch& l, int nv, const void* logits, int64_t ld, void* dlogits, int64_t ldd, const int64_t* labels, const float* lse, const float* coef, const float* dloss,
-                float dloss_mul, int vocab, int64_t ignore_index, const Scale& sc) {
-    const double log2e = (double)sc.lo / sc.inv_tau;   // lse in units of the kernel's x k
-    const int small = (nv + 63) / 64, parts = (nv + 255) / 256;
-    if (nv <= 128) l.parts<64>(logprob_bwd_k<BF, 64, S>, std::max(small, 1), logits, ld, dlogits, ldd, labels, lse, coef, dloss, dloss_mul, vocab, ignore_index, sc, log2e);
-    else l.parts<256>(logprob_bwd_k<BF, 256, S>, parts, logits, ld, dlogits, ldd, labels, lse, coef, dloss, dloss_mul, vocab, ignore_index, sc, log2e);
+template <bool BF, bool L, bool S>
+void launch_bwd(const Launch& l, int nv, const BwdArgs& a, const Scale& sc) {
+    if (nv <= 128) l.parts<64>(logprob_bwd_k<BF, 64, L, S>, std::max((nv + 63) / 64, 1), a, sc);
+    else l.parts<256>(logprob_bwd_k<BF, 256, L, S>, (nv + 255) / 256, a, sc);
 }
 
 // Threads and vectors a thread of the fused kernel, so that the row fills most of them and two workgroups share a CU while they can.  bf16, rows x vocabulary:
@@ -879,10 +912,10 @@ void launch_fused(const Launch& l, int nv, const PolicyArgs& a, const void* logi
     else l.go<1024>(policy_fused_k<BF, 1024, BF ? 10 : 16, true, S>, a, logits, ld, dlogits, ldd, logp, lse, dloss, dloss_mul, sc);
 }
 
-// fn<type, stream>(args...)
-#define IE_ROWS(fn, ...)                                                          \
+// fn<type, past>(args...)
+#define IE_ROWS(fn, past, ...)                                                          \
     do {                                                                          \
-        const bool s_ = streams(rows, vocab, dtype);                              \
+        const bool s_ = past;                                                     \
         const Launch l_ = {(hipStream_t)stream, rows};                            \
         const int nv_ = vectors(vocab, dtype);                                    \
         if (dtype == IE_BF16) {                                                   \
@@ -901,7 +934,7 @@ extern "C" int ie_logprob_fwd(const void* logits, int dtype, int64_t ld, const i
     IE_CHECK_ARG(logits && labels && logp && lse, "ie_logprob_fwd: null pointer");
     IE_CHECK_LOGITS("ie_logprob_fwd");
     if (rows == 0) return IE_OK;
-    IE_ROWS(launch_fwd, logits, ld, labels, logp, lse, (float*)nullptr, (float*)nullptr, (int)vocab, ignore_index, Scale(inv_temperature));
+    IE_ROWS(launch_fwd, beyond(rows, vocab, dtype, false), logits, ld, labels, logp, lse, (float*)nullptr, (float*)nullptr, (int)vocab, ignore_index, Scale(inv_temperature));
     return ie_launch_status("ie_logprob_fwd launch");
 }
 
@@ -911,7 +944,14 @@ extern "C" int ie_logprob_bwd(const void* logits, int dtype, int64_t ld, void* d
     IE_CHECK_LOGITS("ie_logprob_bwd");
     IE_CHECK_ARG(ldd >= vocab && overlap_ok(logits, ld, dlogits, ldd, rows, vocab, dtype), "ie_logprob_bwd: dlogits must be the logits themselves or lie apart from them");
     if (rows == 0) return IE_OK;
-    IE_ROWS(launch_bwd, logits, ld, dlogits, ldd, labels, lse, coef, dloss, dloss_mul, (int)vocab, ignore_index, Scale(inv_temperature));
+    const Scale sc(inv_temperature);
+    const BwdArgs a = {logits, dlogits, ld, ldd, labels, lse, coef, dloss ? dloss : lse, ignore_index, (double)sc.lo / inv_temperature, dloss_mul * (float)inv_temperature,
+                       dloss ? 0.f : 1.f, (int)vocab};
+    const bool loads = beyond(rows, vocab, dtype, false), stores = beyond(rows, vocab, dtype, dlogits != logits);
+    const Launch l = {(hipStream_t)stream, rows};
+    const int nv = vectors(vocab, dtype);
+    if (dtype == IE_BF16) loads ? launch_bwd<true, true, true>(l, nv, a, sc) : stores ? launch_bwd<true, false, true>(l, nv, a, sc) : launch_bwd<true, false, false>(l, nv, a, sc);
+    else loads ? launch_bwd<false, true, true>(l, nv, a, sc) : stores ? launch_bwd<false, false, true>(l, nv, a, sc) : launch_bwd<false, false, false>(l, nv, a, sc);
     return ie_launch_status("ie_logprob_bwd launch");
 }
 
@@ -934,7 +974,7 @@ extern "C" int ie_preference_loss_fwd(const void* logits, int dtype, int64_t ld,
     hipStream_t st = (hipStream_t)stream;
     double* losses = (double*)workspace;
     float* low = (float*)(losses + pairs);
-    if (rows > 0) IE_ROWS(launch_fwd, logits, ld, labels, logp, lse, coef, low, (int)vocab, ignore_index, Scale(inv_temperature));
+    if (rows > 0) IE_ROWS(launch_fwd, beyond(rows, vocab, dtype, false), logits, ld, labels, logp, lse, coef, low, (int)vocab, ignore_index, Scale(inv_temperature));
     const PrefArgs a = {kind, average, beta, label_smoothing, margin};
     const PrefRows r = {logp, low, labels, cu_seqlens, ref_logps, rows, pairs, ignore_index, (int)vocab, rewards, seq_logps, coef};
     if (pairs <= kOnePairs && rows <= kOneRows) {
@@ -973,7 +1013,7 @@ extern "C" int ie_policy_loss(const void* logits, int dtype, int64_t ld, void* d
     a.coef = coef; a.rows = rows; a.seqs = seqs; a.ignore_index = ignore_index; a.vocab = (int)vocab;
     a.low = clip_low; a.high = clip_high; a.kl_coef = kl_coef;
     if (!dlogits && rows <= kSmallRows && seqs <= kSmallSeqs) {
-        if (rows > 0) IE_ROWS(launch_fwd, logits, ld, labels, logp, lse, (float*)nullptr, (float*)nullptr, (int)vocab, ignore_index, Scale(inv_temperature));
+        if (rows > 0) IE_ROWS(launch_fwd, beyond(rows, vocab, dtype, false), logits, ld, labels, logp, lse, (float*)nullptr, (float*)nullptr, (int)vocab, ignore_index, Scale(inv_temperature));
         hipLaunchKernelGGL(policy_small_k, dim3(1), dim3(1024), 0, st, a, (const float*)logp, stats);
         return ie_launch_status("ie_policy_loss launch");
     }
@@ -981,9 +1021,9 @@ extern "C" int ie_policy_loss(const void* logits, int dtype, int64_t ld, void* d
     else if (cu_seqlens) hipLaunchKernelGGL((policy_counts_k<256>), dim3((unsigned)seqs), dim3(256), 0, st, a, counts);
     else hipLaunchKernelGGL((policy_counts_k<1024>), dim3(1), dim3(1024), 0, st, a, counts);
     if (rows > 0 && dlogits) {
-        IE_ROWS(launch_fused, a, logits, ld, dlogits, ldd, logp, lse, dloss, dloss_mul, Scale(inv_temperature));
+        IE_ROWS(launch_fused, beyond(rows, vocab, dtype, dlogits != logits), a, logits, ld, dlogits, ldd, logp, lse, dloss, dloss_mul, Scale(inv_temperature));
     } else if (rows > 0) {
-        IE_ROWS(launch_fwd, logits, ld, labels, logp, lse, (float*)nullptr, (float*)nullptr, (int)vocab, ignore_index, Scale(inv_temperature));
+        IE_ROWS(launch_fwd, beyond(rows, vocab, dtype, false), logits, ld, labels, logp, lse, (float*)nullptr, (float*)nullptr, (int)vocab, ignore_index, Scale(inv_temperature));
         hipLaunchKernelGGL(policy_terms_k, dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, a, (const float*)logp);
     }
     hipLaunchKernelGGL(policy_stats_k, dim3(1), dim3(1024), 0, st, (const float4*)workspace, rows, kl_coef, stats);
