@@ -176,6 +176,20 @@ def test_gradient_of_rows_far_from_zero(dev, centre, temperature, dtype):
         assert torch.equal(inplace, d)
 
 
+@pytest.mark.parametrize("dtype", DTYPES, ids=["bf16", "fp32"])
+def test_log_probabilities_share_no_error(dev, dtype):
+    """Answers of one row each and references next to their log-probabilities: the rewards then show what the log-probabilities are off before they are rounded to
+    32 bits.  Each may be off by a few u; their mean over 8000 rows by 5 u / sqrt(8000) < u / 16 by chance and as much again by what all rows share: a sequence of n
+    rows is off by n times that."""
+    x, y = make(dev, 8000, 5003, dtype, 11, mask=0.0, scale=2.0)
+    z = x.cpu().double()
+    lp = z.gather(1, y.cpu()[:, None])[:, 0] - torch.logsumexp(z, 1)
+    ref = lp.float()
+    r = K().preference_loss_fwd(x, y, torch.arange(8001, dtype=torch.int32, device=dev), ref.to(dev), beta=1.0)
+    off = r.rewards.cpu().double().reshape(-1) - (lp - ref.double())
+    assert float(off.abs().max()) <= 8 * U and abs(float(off.mean())) <= U / 8
+
+
 def pref_ref(logp, labels, cu, ref, beta, kind, eps, margin, average):
     """64-bit loss, rewards, sums and coefficients from given log-probabilities, and what the loss, the rewards and the coefficients may be off: the kernel sums its
     log-probabilities before they are rounded to 32 bits, u |lp| each and all of one sign, so that a sum may be off by u |sum|; the loss by its slope times that, a
