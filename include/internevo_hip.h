@@ -492,12 +492,13 @@ int ie_gemm_set_wgrad_ksplit_workspace(void* ws, int64_t bytes);
  *   z = logits[t] * inv_temperature;  lse[t] = log sum_j exp z_j;  logp[t] = z[labels[t]] - lse[t]
  * logits [rows, vocab] bf16 or fp32, row stride ld, any element address; labels int64 [rows].  A row whose label is ignore_index or lies outside [0, vocab) is
  * masked: its logits are not read, its logp, lse and coef are 0, its gradient row is zeros.  Every [rows] output is written for all rows.
- * ld >= vocab, rows < 2^31, vocab <= 2^30.  No workgroup waits for another and no sum uses atomics: results repeat bit for bit.
+ * ld >= vocab, rows <= 2^26 - 4, vocab <= 2^30, fewer than 2^22 sequences (2^21 pairs); 1e-30 <= inv_temperature <= 1e30.  No workgroup waits for another and no sum uses atomics: results repeat bit for bit.
  *
  * ie_logprob_fwd: logp, lse (fp32 [rows]).
  * ie_logprob_bwd: dlogits[t, j] = g_t ([j == labels[t]] - exp(z_j - lse[t])), g_t = coef[t] * dloss_mul * inv_temperature * (dloss ? *dloss : 1);
  *   coef fp32 [rows] = d loss / d logp, dloss a DEVICE scalar (the loss scale) or NULL.  dlogits has the logits' type and a row stride of its own; it is the
  *   logits themselves (same address, same stride) or does not overlap them.  A row with g_t = 0 is written as zeros without a look at its logits.
+ *   A row whose lse is beyond 128 (fp32) or 2048 (bf16) either way has its sums formed again, since 32 bits of lse no longer hold its probabilities.
  *
  * ie_preference_loss_fwd: cu_seqlens int32 [2 pairs + 1] packs chosen answer 2p and rejected answer 2p + 1; offsets are clamped to [0, rows], rows outside every
  *   sequence are in no sum.  l_s = sum (average: mean; 0 for an answer without a token) of logp over the rows of sequence s that have a label,
