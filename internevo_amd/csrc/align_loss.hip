@@ -339,7 +339,7 @@ __global__ __launch_bounds__(NT) void logprob_fwd_k(const void* __restrict__ log
     }
 }
 
-// `parts` workgroups a row, one vector a thread and no loop: the chip's reads and writes then move through memory as one dense front, which HBM serves at 6.6 TB/s of
+// `parts` workgroups a row, one vector a thread and no loop: the chip's reads and writes then move through memory as one dense front, which HBM serves at 6.2 TB/s of
 // mixed traffic where workgroups that walk a row each get 5.5.  16 384 x 92 544 bf16, 40 % masked: 775 us (a workgroup a row: 871).
 // What a workgroup needs before its first vector is asked for in two rounds, the launch's arguments and then the row's numbers, each as a whole (the compiler would
 // put every scalar load next to its use, six rounds one after the other): with one vector a thread the kernel waits for them longer than it works.

@@ -700,6 +700,8 @@ class MoEEngine:
         self.step_count = ck["adam_step"]
 
     def read_state(self):
+        """Host copy of the step state (synchronises); what the current stream does next finds the parameters of the finished step."""
+        self._wait_optimizer()
         st = K.step_state_read(self.state)
         self.lr_sched.set_successful_steps(st.adam_step)
         self.beta2_sched.set_successful_steps(st.adam_step)
