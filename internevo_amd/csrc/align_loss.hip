@@ -68,17 +68,20 @@ template <bool S> __device__ __forceinline__ void stv(void* p, const u32x4& v) {
 }
 
 // Sums of exponentials.  With k = log2(e) / tau:  exp((x - m) / tau) = 2^(x k - r), r = fl(m k): one fma and one exponential an element, m the largest logit so far; what
-// rounding m k loses is the same factor in every term and goes out again when a thread's sum joins the others'.  The form fails where x k leaves fp32 -- rows in which no
-// logit is above -1e30, such as a vocabulary masked as a whole by the type's lowest value, or whose largest is +inf: those are done over as 2^((x - m) k) (F = false).
-// A maximum that cannot serve counts as none: reference 0, and every term it would belong to is 0 beside any other logit.  NaN and +inf make the sum NaN.
-constexpr float kRange = 1e30f;
-__device__ __forceinline__ float ref(float m, float k) { return m * k >= -kRange ? m * k : 0.f; }
+// rounding m k loses, up to half its last place, is the same factor in every term and goes out again when a thread's sum joins the others'.  That holds while the factor is
+// near 1: up to |m k| = 2^20 it lies within 2^(1/16) either way, at 2^33 it would be 2^512 and the sum lost.  Rows whose maximum lies beyond (logits of 7e5 at a
+// temperature of 1, a vocabulary forbidden as a whole by a finite value, temperatures of 1e-5 and less, a maximum of +inf or -inf) are done over as 2^((x - m) k) (F = false).  NaN and +inf make the sum NaN.
+// A thread whose own maximum lies below -2^21 gets the reference 0, and its terms are 0 as they should be beside a row maximum above -2^20; between the two
+// bounds it is joined like any other.
+constexpr float kRange = 1048576.f, kLow = -2097152.f;
+__device__ __forceinline__ bool counts(float m, float k) { return m * k >= kLow; }   // (false for NaN)
+__device__ __forceinline__ float ref(float m, float k) { return counts(m, k) ? m * k : 0.f; }
 __device__ __forceinline__ bool in_range(float m, float k) { return fabsf(m * k) <= kRange; }
 template <bool F> __device__ __forceinline__ float term(float x, float k, float r) { return exp2_(F ? __builtin_fmaf(x, k, -r) : (x - r) * k); }
 
 // Sums of hundreds of log-probabilities show any error that all rows share.  The hardware's exponential is 3.3e-9 low on average (measured: every argument range from
 // [-1, 0) to [-30, -29) the same to 1 %), which log_sum below puts right for the terms; what multiplies a whole sum uses this instead:
-// 2^d for d <= 0 by the Taylor series of 2^f, |f| <= 1/2, off by 2e-10, and one rounding to the nearest.
+// 2^d for d <= 0 by the Taylor series of 2^f, off by 2e-10 for |f| <= 1/2 (by 2e-9 at 5/8, the most that what a thread's reference lost adds), and one rounding to the nearest.
 constexpr double kExpLow = 3.3e-9;
 __device__ __forceinline__ float exp2_near(float f, float n) {   // 2^(f + n), n whole
     float p = 1.3215486790e-6f;
@@ -798,7 +801,7 @@ __global__ __launch_bounds__(NT, NT >= 512 ? 4 : 1) void policy_fused_k(PolicyAr
         s += tree_sum<N>(ex + j * N);
     }
     RowStat st = join_stats<NT>(m, s, k, sc, sh);
-    own = m * k >= -kRange ? to_max(m, k, st.m, sc) : 0.f;   // now: the factor of the thread's terms
+    own = counts(m, k) ? to_max(m, k, st.m, sc) : 0.f;   // now: the factor of the thread's terms
     if (!st.fast) st = row_stat_again<BF, NT>(x, vocab, st.m, sc.lo, sh);
     if (!a.counts) {
 #pragma unroll
