@@ -456,7 +456,8 @@ __device__ __forceinline__ double pair_loss(const PrefArgs& a, double h, double&
     const double z = a.beta * h - a.margin;
     if (a.kind == IE_PREF_SIGMOID) {
         slope = a.beta * (a.smoothing / (1.0 + exp(-z)) - (1.0 - a.smoothing) / (1.0 + exp(z)));
-        return -(1.0 - a.smoothing) * log_sigmoid(z) - a.smoothing * log_sigmoid(-z);
+        const double right = -(1.0 - a.smoothing) * log_sigmoid(z);
+        return a.smoothing > 0.0 ? right - a.smoothing * log_sigmoid(-z) : right;   // (0 * inf would turn a pair that is infinitely right into NaN)
     }
     if (a.kind == IE_PREF_HINGE) {
         slope = z < 1.0 ? -a.beta : z == z ? 0.0 : z;

@@ -167,3 +167,43 @@ def test_logits_far_from_zero(dev, centre, V, dtype):
     x = (torch.randn(8, V, generator=g) * 3 + centre).to(dtype).to(dev)
     x[:4, :V // 3] -= abs(centre) / 16
     everything(dev, x, x.argmax(1), 1.0)
+
+
+def pair_formula(kind, eps, beta, h):
+    """loss and its slope in h of one pair, infinite log-ratios as limits"""
+    z = beta * h
+    sig = 0.0 if z == -math.inf else 1.0 / (1.0 + math.exp(-z)) if z > -700 else math.exp(z)
+    if kind == "sigmoid":
+        soft = [math.inf if v == math.inf else 0.0 if v == -math.inf else max(v, 0.0) + math.log1p(math.exp(-abs(v))) for v in (-z, z)]
+        return (1 - eps) * soft[0] + (eps * soft[1] if eps else 0.0), beta * (eps * sig - (1 - eps) * (1.0 - sig))
+    if kind == "hinge":
+        return max(0.0, 1.0 - z), -beta if z < 1 else 0.0
+    return (h - 0.5 / beta) ** 2, 2 * (h - 0.5 / beta)
+
+
+FORMS = [("sigmoid", 0.0), ("sigmoid", 0.2), ("hinge", 0.0), ("ipo", 0.0)]
+
+
+@pytest.mark.parametrize("pairs", [1, 2, 3, 7, 9])
+@pytest.mark.parametrize("kind, eps", FORMS)
+@pytest.mark.parametrize("where, value", [(0, -math.inf), (0, math.inf), (1, -math.inf), (1, math.inf)])
+def test_infinite_reference_log_probabilities(dev, where, value, kind, eps, pairs):
+    """The log-ratio of the last pair is infinite: its loss is 0 or infinite, its slope a limit, and the other pairs are as they were."""
+    rows, V, beta = 6 * pairs, 211, 0.4
+    g = torch.Generator().manual_seed(pairs)
+    x, y = torch.randn(rows, V, generator=g).to(dev), torch.randint(0, V, (rows,), generator=g).to(dev)
+    cu = torch.arange(0, rows + 1, 3, dtype=torch.int32, device=dev)
+    lp = Ref(x, y, 1.0)
+    ref = lp.logp.reshape(-1, 3).sum(1).float() + torch.randn(2 * pairs, generator=g)
+    ref[2 * pairs - 2 + where] = value
+    r = K().preference_loss_fwd(x, y, cu, ref.to(dev), beta=beta, kind=kind, label_smoothing=eps)
+    gain = lp.logp.reshape(-1, 3).sum(1) - ref.double()
+    each = [pair_formula(kind, eps, beta, float(a - b)) for a, b in gain.reshape(-1, 2)]
+    off = float(lp.logp_tol.reshape(-1, 6).sum(1).max())      # of a pair's log-ratio
+    steep = max(abs(s) for _, s in each if math.isfinite(s)) if any(math.isfinite(s) for _, s in each) else 0.0
+    loss = sum(v for v, _ in each) / pairs
+    check(r.loss, torch.tensor([loss]), steep * off + 2 * U * abs(loss) + 1e-12, "loss")
+    coef = torch.tensor([[s] * 3 + [-s] * 3 for _, s in each]).double().reshape(-1) / pairs
+    bend = {"sigmoid": beta ** 2 / 4, "hinge": 0.0, "ipo": 2.0}[kind]
+    check(r.coef, coef, (bend * off + 2 * U * coef.abs() + 2.0 ** -50), "coef")
+    check(r.rewards.reshape(-1), beta * gain, beta * off + 2 * U * beta * gain.abs(), "rewards")
