@@ -337,8 +337,9 @@ __global__ __launch_bounds__(NT) void logprob_fwd_k(const void* __restrict__ log
     if (threadIdx.x == 0) {
         const double lp = st.logp(xl, sc.inv_tau);
         lse[row] = (float)st.lse(sc.inv_tau);
-        logp[row] = (float)lp;
-        if (coef) { coef[row] = 0.f; low[row] = (float)(lp - (double)(float)lp); }
+        const float l = (float)lp;
+        logp[row] = l;
+        if (coef) { coef[row] = 0.f; low[row] = fabsf(l) < INFINITY ? (float)(lp - (double)l) : 0.f; }   // (a label of logit -inf: nothing is lost, and inf - inf is NaN)
     }
 }
 

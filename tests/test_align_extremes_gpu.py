@@ -207,3 +207,38 @@ def test_infinite_reference_log_probabilities(dev, where, value, kind, eps, pair
     bend = {"sigmoid": beta ** 2 / 4, "hinge": 0.0, "ipo": 2.0}[kind]
     check(r.coef, coef, (bend * off + 2 * U * coef.abs() + 2.0 ** -50), "coef")
     check(r.rewards.reshape(-1), beta * gain, beta * off + 2 * U * beta * gain.abs(), "rewards")
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=["bf16", "fp32"])
+@pytest.mark.parametrize("pairs", [1, 3, 9])
+@pytest.mark.parametrize("average", [False, True], ids=["sums", "means"])
+@pytest.mark.parametrize("kind, eps", FORMS)
+@pytest.mark.parametrize("where", [0, 1], ids=["chosen", "rejected"])
+def test_a_label_whose_logit_is_minus_infinity(dev, where, kind, eps, average, pairs, dtype):
+    """One token of the first pair is impossible (log-probability -inf): its answer's sum is -inf, the pair's loss 0 or infinite with the slope's limit, and gradients of
+    finite slopes are finite."""
+    rows, V, beta = 6 * pairs, 1031, 0.4
+    g = torch.Generator().manual_seed(pairs)
+    x, y = (torch.randn(rows, V, generator=g) * 2).to(dtype).to(dev), torch.randint(0, V, (rows,), generator=g).to(dev)
+    bad = 3 * where + 1
+    x[bad, y[bad]] = -math.inf
+    cu = torch.arange(0, rows + 1, 3, dtype=torch.int32, device=dev)
+    n = 3 if average else 1
+    r = K().preference_loss_fwd(x, y, cu, beta=beta, kind=kind, label_smoothing=eps, average=average)
+    lp = Ref(x, y, 1.0)
+    check(r.logp, lp.logp, lp.logp_tol, "logp")
+    sums = lp.logp.reshape(-1, 3).sum(1) / n
+    tol = lp.sum_tol.reshape(-1, 3).sum(1) + 2 * U * torch.where(torch.isfinite(sums), sums.abs(), torch.zeros(()))
+    check(r.seq_logps, sums, tol, "seq_logps")
+    check(r.rewards.reshape(-1), beta * sums, beta * tol + 2 * U * beta * sums.abs(), "rewards")
+    each = [pair_formula(kind, eps, beta, float(a - b)) for a, b in sums.reshape(-1, 2)]
+    off = float(tol.reshape(-1, 2).sum(1).max())
+    steep = max([abs(s) for _, s in each if math.isfinite(s)] or [0.0])
+    loss = sum(v for v, _ in each) / pairs
+    check(r.loss, torch.tensor([loss]), steep * off + 2 * U * abs(loss) + 1e-12, "loss")
+    coef = torch.tensor([[s] * 3 + [-s] * 3 for _, s in each]).double().reshape(-1) / pairs / n
+    bend = {"sigmoid": beta ** 2 / 4, "hinge": 0.0, "ipo": 2.0}[kind]
+    check(r.coef, coef, bend * off + 2 * U * coef.abs() + 2.0 ** -50, "coef")
+    if kind != "ipo":
+        d = K().preference_loss_bwd(x, y, r, torch.full((1,), 8.0, device=dev), dlogits=torch.full_like(x, 7.0))
+        lp.check_dlogits(d, r.coef.double() * 8.0, "dlogits")
