@@ -665,6 +665,7 @@ __global__ __launch_bounds__(256) void policy_terms_k(PolicyArgs a, const float*
 
 // sums of the three terms over a workgroup of 1024 threads (scratch: 48 doubles) -> loss, surrogate, KL, clipped share
 __device__ __forceinline__ void write_stats(double* v, float kl_coef, float* stats, double* scratch) {
+    __syncthreads();   // (scratch may hold an earlier sum that other waves still read)
 #pragma unroll
     for (int c = 0; c < 3; ++c) {
         v[c] = wave_sum_d(v[c]);

@@ -242,3 +242,21 @@ def test_a_label_whose_logit_is_minus_infinity(dev, where, kind, eps, average, p
     if kind != "ipo":
         d = K().preference_loss_bwd(x, y, r, torch.full((1,), 8.0, device=dev), dlogits=torch.full_like(x, 7.0))
         lp.check_dlogits(d, r.coef.double() * 8.0, "dlogits")
+
+
+@pytest.mark.parametrize("rows", [1, 63, 1000, 4095, 4096])
+def test_short_batches_weigh_every_row_alike(dev, rows):
+    """The one workgroup that finishes a short batch counts its tokens and sums its terms in the same shared memory: every call gives the same bits, those of the batch as one
+    sequence, whose weights 1 / (1 N) are the same numbers."""
+    V = 17
+    g = torch.Generator().manual_seed(rows)
+    x, y = torch.randn(rows, V, generator=g).to(dev), torch.randint(0, V, (rows,), generator=g)
+    y[torch.rand(rows, generator=g) < 0.3] = IGNORE
+    y[0] = 3
+    y = y.to(dev)
+    old, adv, ref = (torch.randn(rows, generator=g).to(dev) for _ in range(3))
+    old, ref = old * 0.1 - 2.8, ref * 0.1 - 2.8
+    want = K().policy_loss_fwd(x, y, old, adv, ref, kl_coef=0.1, cu_seqlens=torch.tensor([0, rows], dtype=torch.int32, device=dev))
+    for _ in range(50):
+        got = K().policy_loss_fwd(x, y, old, adv, ref, kl_coef=0.1)
+        assert torch.equal(got.coef, want.coef) and torch.equal(got.stats, want.stats)
