@@ -645,7 +645,7 @@ __device__ __forceinline__ float policy_term(const PolicyArgs& a, const PolicyRo
     float d = clipped ? 0.f : -ratio * in.adv, kl = 0.f;
     if (a.ref) {
         const float q = (float)((double)in.ref - logp), e = expm1f(q);
-        kl = e - q;
+        kl = e == INFINITY ? e : e - q;   // (a label of logit -inf: q is inf too, and inf - inf is NaN)
         if (a.kl_coef > 0.f) d -= a.kl_coef * e;   // (0 * inf would turn a mere report into NaN)
     }
     term = make_float4(w * s, w * kl, clipped ? w : 0.f, 0.f);

@@ -260,3 +260,40 @@ def test_short_batches_weigh_every_row_alike(dev, rows):
     for _ in range(50):
         got = K().policy_loss_fwd(x, y, old, adv, ref, kl_coef=0.1)
         assert torch.equal(got.coef, want.coef) and torch.equal(got.stats, want.stats)
+
+
+def policy_forms(dev, x, y, old, adv, ref, kl_coef):
+    """The same rows, one sequence, through every form"""
+    cu = torch.tensor([0, x.shape[0]], dtype=torch.int32, device=dev)
+    one = torch.ones(1, device=dev)
+    args = dict(ref_logps=ref, kl_coef=kl_coef)
+    yield "small batch", K().policy_loss_fwd(x, y, old, adv, cu_seqlens=cu, **args)
+    long = 4097 - x.shape[0]      # masked rows behind the sequence: past the rows that one workgroup finishes
+    more = lambda t, v: torch.cat([t, torch.full((long, *t.shape[1:]), v, dtype=t.dtype, device=dev)])   # noqa: E731
+    yield "long batch", K().policy_loss_fwd(more(x, 0.0), more(y, IGNORE), more(old, 0.0), more(adv, 0.0), ref_logps=more(ref, 0.0), kl_coef=kl_coef, cu_seqlens=cu)
+    yield "one pass", K().policy_loss_fwd_bwd(x, y, old, adv, one, dlogits=torch.empty_like(x), cu_seqlens=cu, **args)[0]
+
+
+def policy_rows(dev, seed):
+    rows, V = 6, 300
+    g = torch.Generator().manual_seed(seed)
+    x, y = torch.randn(rows, V, generator=g).to(dev), torch.randint(0, V, (rows,), generator=g).to(dev)
+    lp = Ref(x, y, 1.0).logp
+    return x, y, (lp - 0.05).float().to(dev), torch.tensor([0.5, 1.0, -1.0, 0.75, -0.5, 2.0], device=dev), (lp + 0.2).float().to(dev)
+
+
+@pytest.mark.parametrize("kl_coef", [0.0, 0.1])
+def test_kl_of_an_impossible_label(dev, kl_coef):
+    """exp(q) - q - 1 of q = inf is inf, reported and in the loss; without a weight on it the loss and every coefficient stay as they are."""
+    x, y, old, adv, ref = policy_rows(dev, 1)
+    for what, base in policy_forms(dev, x, y, old, adv, ref, kl_coef):
+        assert bool(torch.isfinite(base.stats).all()), what
+    x[1, y[1]] = -math.inf
+    for what, r in policy_forms(dev, x, y, old, adv, ref, kl_coef):
+        assert float(r.logp[1]) == -math.inf and float(r.stats[2]) == math.inf, (what, r.stats)
+        if kl_coef:
+            assert float(r.stats[0]) == math.inf and float(r.coef[1]) == -math.inf, (what, r.stats)
+        else:
+            assert bool(torch.isfinite(r.stats[[0, 1, 3]]).all()) and float(r.coef[1]) == 0.0, (what, r.stats)
+        rest = [0, 2, 3, 4, 5]
+        assert bool(torch.isfinite(r.coef[rest]).all()) and bool((r.coef[rest] != 0).all()), what
