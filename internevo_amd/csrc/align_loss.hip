@@ -641,8 +641,9 @@ __device__ __forceinline__ float policy_term(const PolicyArgs& a, const PolicyRo
     const float ratio = expf((float)(logp - (double)in.old));
     const bool clipped = (in.adv > 0.f && ratio > 1.f + a.high) || (in.adv < 0.f && ratio < 1.f - a.low);
     const float bound = in.adv > 0.f ? 1.f + a.high : 1.f - a.low;
-    const float s = -(clipped ? bound : ratio) * in.adv;
-    float d = clipped ? 0.f : -ratio * in.adv, kl = 0.f;
+    const float gain = ratio == INFINITY && in.adv == 0.f ? 0.f : ratio * in.adv;   // (a ratio past fp32 without an advantage adds nothing)
+    const float s = -(clipped ? bound * in.adv : gain);
+    float d = clipped ? 0.f : -gain, kl = 0.f;
     if (a.ref) {
         const float q = (float)((double)in.ref - logp), e = expm1f(q);
         kl = e == INFINITY ? e : e - q;   // (a label of logit -inf: q is inf too, and inf - inf is NaN)

@@ -297,3 +297,16 @@ def test_kl_of_an_impossible_label(dev, kl_coef):
             assert bool(torch.isfinite(r.stats[[0, 1, 3]]).all()) and float(r.coef[1]) == 0.0, (what, r.stats)
         rest = [0, 2, 3, 4, 5]
         assert bool(torch.isfinite(r.coef[rest]).all()) and bool((r.coef[rest] != 0).all()), what
+
+
+def test_ratio_past_fp32_without_an_advantage(dev):
+    """r A = 0 where A = 0, whatever the ratio is: the row adds its KL term alone."""
+    x, y, old, adv, ref = policy_rows(dev, 2)
+    adv[3] = 0.0
+    want = {what: r for what, r in policy_forms(dev, x, y, old, adv, ref, 0.1)}
+    old[3] = -200.0
+    for what, r in policy_forms(dev, x, y, old, adv, ref, 0.1):
+        assert torch.equal(r.coef, want[what].coef) and torch.equal(r.stats, want[what].stats), (what, r.stats, want[what].stats)
+    x[3, 5] = math.nan
+    for what, r in policy_forms(dev, x, y, old, adv, ref, 0.1):
+        assert bool(r.stats[0].isnan()) and bool(r.coef[3].isnan()), what
