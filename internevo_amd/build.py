@@ -1,6 +1,6 @@
 """Build libinternevo_hip.so (and the oracle's C pieces, if any) in-tree with hipcc for gfx950.
 
-hipcc cross-compiles without a GPU.  Objects are cached by source mtime so rebuilding after a
+hipcc cross-compiles without a GPU.  Objects are cached by source mtime and flags so rebuilding after a
 one-file edit takes seconds.  The .so is git-ignored but travels to the GPU box with the snapshot.
 """
 import concurrent.futures
@@ -42,17 +42,29 @@ def _headers_mtime():
     return max(os.path.getmtime(h) for h in hs)
 
 
+def _read(path):
+    if not os.path.exists(path):
+        return None
+    with open(path) as f:
+        return f.read()
+
+
 def _compile(src, force):
     obj = os.path.join(OBJ, src.replace(".hip", ".o"))
     spath = os.path.join(CSRC, src)
-    if not force and os.path.exists(obj) and os.path.getmtime(obj) > max(os.path.getmtime(spath), _headers_mtime()):
+    flags = [*FLAGS, *EXTRA_FLAGS.get(src, [])]
+    record, made_with = obj[:-2] + ".flags", "\n".join(flags)   # what the object beside it was built with
+    if not force and os.path.exists(obj) and os.path.getmtime(obj) > max(os.path.getmtime(spath), _headers_mtime()) and _read(record) == made_with:
         return obj, False
-    cmd = [_hipcc(), *FLAGS, *EXTRA_FLAGS.get(src, []), "-c", spath, "-o", obj]
-    if os.path.exists(obj):
-        os.remove(obj)  # a stale object must never survive a failed compile (the hipcc wrapper can exit 0 after "failed to execute")
+    cmd = [_hipcc(), *flags, "-c", spath, "-o", obj]
+    for stale in (obj, record):
+        if os.path.exists(stale):
+            os.remove(stale)  # a stale object must never survive a failed compile (the hipcc wrapper can exit 0 after "failed to execute")
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0 or not os.path.exists(obj) or "error:" in res.stderr:
         raise RuntimeError(f"hipcc failed for {src}:\n{res.stdout}\n{res.stderr}")
+    with open(record, "w") as f:
+        f.write(made_with)
     return obj, True
 
 
