@@ -4,6 +4,8 @@ hipcc cross-compiles without a GPU.  Objects are cached by source mtime and flag
 one-file edit takes seconds.  The .so is git-ignored but travels to the GPU box with the snapshot.
 """
 import concurrent.futures
+import contextlib
+import fcntl
 import os
 import shutil
 import subprocess
@@ -70,6 +72,13 @@ def _compile(src, force):
 
 def build(force=False, verbose=True):
     os.makedirs(OBJ, exist_ok=True)
+    with contextlib.ExitStack() as stack:
+        if os.access(OBJ, os.W_OK):   # two programs that find something to build do it one after the other (a tree that cannot be written has nothing to build)
+            fcntl.flock(stack.enter_context(open(os.path.join(OBJ, "lock"), "a")), fcntl.LOCK_EX)
+        return _build(force, verbose)
+
+
+def _build(force, verbose):
     srcs = _sources()
     with concurrent.futures.ThreadPoolExecutor(max_workers=min(8, len(srcs))) as ex:
         results = list(ex.map(lambda s: _compile(s, force), srcs))

@@ -74,3 +74,27 @@ def test_a_changed_source_is_compiled_again(tree):
 def test_packed_fp32_arithmetic_is_off_for_every_source():
     at = B.FLAGS.index("-packed-fp32-ops")
     assert B.FLAGS[at - 3:at] == ["-Xclang", "-target-feature", "-Xclang"]
+
+
+def test_two_programs_build_one_after_the_other(tree):
+    """The second waits and finds everything up to date, where it used to remove objects that the first was linking."""
+    import multiprocessing
+    import time
+
+    tmp_path, _ = tree
+    real, start = B._compile, multiprocessing.get_context("fork")
+
+    def slow(src, force):
+        time.sleep(0.3)
+        return real(src, force)
+
+    B._compile = slow
+    try:
+        (tmp_path / "calls").write_text("")
+        ps = [start.Process(target=B.build, kwargs=dict(verbose=False)) for _ in range(2)]
+        [p.start() for p in ps]
+        [p.join(60) for p in ps]
+    finally:
+        B._compile = real
+    assert [p.exitcode for p in ps] == [0, 0]
+    assert sorted(os.path.basename(c) for c in (tmp_path / "calls").read_text().split() if c.endswith(".hip")) == ["one.hip", "two.hip"]
