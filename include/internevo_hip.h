@@ -497,7 +497,7 @@ int ie_gemm_set_wgrad_ksplit_workspace(void* ws, int64_t bytes);
  * ie_logprob_fwd: logp, lse (fp32 [rows]).
  * ie_logprob_bwd: dlogits[t, j] = g_t ([j == labels[t]] - exp(z_j - lse[t])), g_t = coef[t] * dloss_mul * inv_temperature * (dloss ? *dloss : 1);
  *   coef fp32 [rows] = d loss / d logp, dloss a DEVICE scalar (the loss scale) or NULL.  dlogits has the logits' type and a row stride of its own; it is the
- *   logits themselves (same address, same stride) or does not overlap them.  A row with g_t = 0 is written as zeros without a look at its logits.
+ *   logits themselves (same address, same stride) or lies before or behind all their rows.  A row with g_t = 0 is written as zeros without a look at its logits.
  *   A row whose lse is beyond 128 (fp32) or 2048 (bf16) either way has its sums formed again, since 32 bits of lse no longer hold its probabilities.
  *
  * ie_preference_loss_fwd: cu_seqlens int32 [2 pairs + 1] packs chosen answer 2p and rejected answer 2p + 1; offsets are clamped to [0, rows], rows outside every
@@ -507,12 +507,14 @@ int ie_gemm_set_wgrad_ksplit_workspace(void* ws, int64_t bytes);
  *     IE_PREF_HINGE    max(0, 1 - z)
  *     IE_PREF_IPO      (h - 1 / (2 beta))^2                          (no margin)
  *   loss[0] = mean over the pairs; rewards [2 pairs] = beta (l - ref); seq_logps [2 pairs] = l; coef [rows] = d loss / d logp for ie_logprob_bwd.
+ *   A label of logit -inf has logp -inf and makes its answer's sum -inf; losses and slopes of an infinite h are the formulas' limits.
  *   Sums and losses are formed in 64 bits, from log-probabilities that are not rounded to 32 first.  workspace: ie_preference_loss_workspace(rows, pairs) bytes, 8-byte aligned, for this call only.
  *
  * ie_policy_loss: r = exp(logp - old_logps), loss term -min(r A, clamp(r, 1 - clip_low, 1 + clip_high) A) + kl_coef (exp(q) - q - 1), q = ref_logps - logp
  *   (ref_logps NULL: no KL term, kl_coef must be 0); old_logps, advantages, ref_logps fp32 [rows], not looked at in masked rows.  Weights: cu_seqlens NULL
  *   (seqs = 0): 1 / N over the N rows with a label; cu_seqlens int32 [seqs + 1]: 1 / (seqs n_s) for the n_s labelled rows of sequence s, 0 outside every sequence.
- *   stats[4] = {loss, policy term, KL, share of clipped rows} under those weights (all 0 for a batch without a label); logp, lse, coef as above.
+ *   stats[4] = {loss, policy term, KL, share of clipped rows} under those weights (all 0 for a batch without a label; a label of logit -inf has the KL inf, A = 0 adds no policy term
+ *   whatever r is); logp, lse, coef as above.
  *   dlogits and dloss given: the gradient too, in the same pass over the logits (dlogits as in ie_logprob_bwd); both NULL: forward only, ie_logprob_bwd follows.
  *   workspace: ie_policy_loss_workspace(rows, seqs) bytes, 16-byte aligned, for this call only.
  * ---------------------------------------------------------------------------------------------- */
@@ -543,6 +545,7 @@ int ie_policy_loss(const void* logits, int dtype, int64_t ld, void* dlogits, int
  * ie_grad_clip: norm[0] the same, then out_i = g_i * c, c = min(1, max_norm / (norm[0] + 1e-6)) (torch.nn.utils.clip_grad_norm_'s rule: an infinite norm gives
  *   c = 0, a NaN one c = NaN).  outs NULL: in place (nothing is moved when c = 1; tensors must not overlap); else outs[i] of out_dtypes[i] and numels[i] elements,
  *   apart from every other tensor of the call, or the same one as ptrs[i].
+ *   The norm is the list's own: where ranks or pipeline stages hold parts of a model, each would clip by another factor.
  * ---------------------------------------------------------------------------------------------- */
 int64_t ie_grad_norm_workspace(int64_t n);
 int ie_grad_norm(const void* const* ptrs, const int64_t* numels, const int* dtypes, int64_t n, void* workspace, float* norm, void* stream);

@@ -70,12 +70,13 @@ template <bool S> __device__ __forceinline__ void stv(void* p, const u32x4& v) {
 // Sums of exponentials.  With k = log2(e) / tau:  exp((x - m) / tau) = 2^(x k - r), r = fl(m k): one fma and one exponential an element, m the largest logit so far; what
 // rounding m k loses, up to half its last place, is the same factor in every term and goes out again when a thread's sum joins the others'.  That holds while the factor is
 // near 1: up to |m k| = 2^20 it lies within 2^(1/16) either way, at 2^33 it would be 2^512 and the sum lost.  Rows whose maximum lies beyond (logits of 7e5 at a
-// temperature of 1, a vocabulary forbidden as a whole by a finite value, temperatures of 1e-5 and less, a maximum of +inf or -inf) are done over as 2^((x - m) k) (F = false).  NaN and +inf make the sum NaN.
+// temperature of 1, a vocabulary forbidden as a whole by a finite value, temperatures of 1e-5 and less, a maximum of +inf or -inf) are done over as
+// 2^((x - m) k) (F = false).  NaN and +inf make the sum NaN.
 // A thread whose own maximum lies below -2^21 gets the reference 0, and its terms are 0 as they should be beside a row maximum above -2^20; between the two
 // bounds it is joined like any other.
 constexpr float kRange = 1048576.f, kLow = -2097152.f;
-__device__ __forceinline__ bool counts(float m, float k) { return m * k >= kLow; }   // (false for NaN)
-__device__ __forceinline__ float ref(float m, float k) { return counts(m, k) ? m * k : 0.f; }
+__device__ __forceinline__ bool usable(float m, float k) { return m * k >= kLow; }   // (false for NaN)
+__device__ __forceinline__ float ref(float m, float k) { return usable(m, k) ? m * k : 0.f; }
 __device__ __forceinline__ bool in_range(float m, float k) { return fabsf(m * k) <= kRange; }
 template <bool F> __device__ __forceinline__ float term(float x, float k, float r) { return exp2_(F ? __builtin_fmaf(x, k, -r) : (x - r) * k); }
 
@@ -805,7 +806,7 @@ __global__ __launch_bounds__(NT, NT >= 512 ? 4 : 1) void policy_fused_k(PolicyAr
         s += tree_sum<N>(ex + j * N);
     }
     RowStat st = join_stats<NT>(m, s, k, sc, sh);
-    own = counts(m, k) ? to_max(m, k, st.m, sc) : 0.f;   // now: the factor of the thread's terms
+    own = usable(m, k) ? to_max(m, k, st.m, sc) : 0.f;   // now: the factor of the thread's terms
     if (!st.fast) st = row_stat_again<BF, NT>(x, vocab, st.m, sc.lo, sh);
     if (!a.counts) {
 #pragma unroll

@@ -386,7 +386,8 @@ def _dlogits_for(logits, dlogits):
 
 def token_logprobs(logits, labels, ignore_index=-100, temperature=1.0):
     """logits [rows, V] (bf16|fp32, row stride arbitrary), labels int64 [rows] -> (logp, lse) fp32 [rows]: the log-probability of every row's label under
-    softmax(logits / temperature) and the row's log-sum-exp.  Rows whose label is ignore_index or no column are masked: both values are 0."""
+    softmax(logits / temperature) and the row's log-sum-exp.  Rows whose label is ignore_index or no column are masked: both values are 0
+    (so the parts of a vocabulary that is split over ranks cannot be joined from them)."""
     rows, V, ld = _logit_rows(logits)
     _row_vector(labels, rows, torch.int64, "labels")
     inv = _inv_temperature(temperature)
@@ -568,7 +569,8 @@ def grad_norm(tensors):
 def clip_grad_norm_(tensors, max_norm, out=None):
     """Scales the gradients by min(1, max_norm / (norm + 1e-6)) (torch.nn.utils.clip_grad_norm_'s rule, its non-finite norms too) and returns their norm before that,
     fp32[1] on the device; no host synchronisation.  In place, or into `out`: a list of contiguous tensors of the same lengths, bf16 or fp32 (the optimizer's fp32
-    gradients), apart from the inputs.  A tensor named twice, or overlapping another one that is written, is refused."""
+    gradients), apart from the inputs.  A tensor named twice, or overlapping another one that is written, is refused.  The norm is this list's own: ranks or stages that hold
+    parts of a model would each clip by another factor."""
     tensors = list(tensors)
     if not max_norm >= 0:
         raise ValueError(f"clip_grad_norm_: max_norm must not be negative ({max_norm})")
